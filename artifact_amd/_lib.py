@@ -21,6 +21,7 @@ SYMBOLS = (
     "rof_layout_export", "rof_layout_stats", "rof_layout_upload", "rof_layout_set_degrees",
     "rof_plan_hub_patterns", "rof_plan_dynamic_greedy", "rof_column_sums", "rof_column_sums_workspace_bytes", "rof_layout_workspace_bytes", "rof_layout_free", "rof_aggregate", "rof_aggregate_epilogue", "rof_aggregate_noalloc", "rof_aggregate_timed", "rof_aggregate_launch_times",
     "rof_device_copy", "rof_device_read", "rof_device_gather", "rof_layout_set_tuning", "rof_layout_get_tuning", "rof_layout_stats_n", "rof_layout_calibrate",
+    "rof_dropout", "rof_dropout_state_next", "rof_layer_norm", "rof_layer_norm_backward", "rof_layer_norm_backward_workspace_bytes",
 )
 
 
@@ -43,6 +44,10 @@ class LaunchTuning(C.Structure):
 class Epilogue(C.Structure):
     _fields_ = [("bias", C.c_void_p), ("relu", C.c_int32), ("out_dtype", C.c_int32), ("self_weight", C.c_float),
                 ("pad_columns", C.c_int32), ("reserved", C.c_int32 * 2)]
+
+
+class DropoutOpts(C.Structure):
+    _fields_ = [("p", C.c_double), ("state", C.c_void_p), ("call", C.c_int64)]
 
 
 def lib():
@@ -99,6 +104,14 @@ def lib():
     L.rof_device_copy.argtypes = [vp, vp, C.c_size_t, vp]
     L.rof_aggregate_launch_times.argtypes = [vp, vp, ci, i64, vp, i64, ci, ci, C.POINTER(Epilogue), vp, C.c_size_t, vp, ci,
                                              C.POINTER(C.c_float * 2)]
+    f64, drop = C.c_double, C.POINTER(DropoutOpts)
+    L.rof_dropout.argtypes = [vp, ci, i64, i64, ci, vp, i64, drop, vp]
+    L.rof_dropout_state_next.argtypes = [vp, i64, vp, vp]
+    L.rof_layer_norm.argtypes = [vp, ci, i64, i64, ci, vp, vp, f64, ci, drop, vp, ci, i64, vp]
+    L.rof_layer_norm_backward_workspace_bytes.restype = C.c_size_t
+    L.rof_layer_norm_backward_workspace_bytes.argtypes = [i64, ci]
+    L.rof_layer_norm_backward.argtypes = [vp, ci, i64, vp, ci, i64, i64, ci, vp, vp, f64, ci, drop, vp, i64, vp, vp, vp,
+                                          C.c_size_t, vp]
     _lib = L
     return L
 

@@ -12,15 +12,6 @@
 #include "rof.h"
 #include "rof_internal.h"
 
-#define HIP_TRY(expr)                                                                  \
-    do {                                                                               \
-        hipError_t e_ = (expr);                                                        \
-        if (e_ != hipSuccess) {                                                        \
-            rof_set_device_error(#expr, hipGetErrorString(e_));                        \
-            return ROF_ERR_DEVICE;                                                     \
-        }                                                                              \
-    } while (0)
-
 namespace rofk {
 
 struct AggArgs {

@@ -77,4 +77,13 @@ struct rof_layout {
 
 void rof_set_device_error(const char *what, const char *text);
 
+#define HIP_TRY(expr)                                                                  \
+    do {                                                                               \
+        hipError_t e_ = (expr);                                                        \
+        if (e_ != hipSuccess) {                                                        \
+            rof_set_device_error(#expr, hipGetErrorString(e_));                        \
+            return ROF_ERR_DEVICE;                                                     \
+        }                                                                              \
+    } while (0)
+
 #endif

@@ -1,0 +1,249 @@
+// Operators on the feature rows between two graph convolutions: layer norm (forward, backward; kernels in norm_rows.h),
+// dropout whose mask is computed and never stored, and the generator state the dropout reads.  C ABI in include/rof.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "rof.h"
+#include "rof_internal.h"
+#include "row_ops.h"
+
+namespace {
+
+using namespace rofn;
+
+constexpr int kMaxNormColumns = ROF_LAYER_NORM_MAX_COLUMNS;
+// Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.
+constexpr int kBackwardBlocks = 1024;
+constexpr int kForwardBlocks = 2048;
+
+struct DropoutArgs {
+    const void *x;
+    void *out;
+    int64_t ldx, ldo;
+    int64_t items;           // rows times groups of eight columns
+    int32_t f, groups;
+    uint32_t threshold;
+    float scale;
+    const int64_t *state;
+    int64_t call;
+};
+
+// One thread per group of eight columns, that is per call of the generator.
+template <typename T>
+__global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
+    const Drop d(a);
+    const int64_t step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.items; i += step) {
+        const int64_t row = i / a.groups;
+        const int col = (int)(i - row * a.groups) * 8, left = a.f - col;
+        const T *src = (const T *)a.x + row * a.ldx + col;
+        T *dst = (T *)a.out + row * a.ldo + col;
+        uint32_t w[4];
+        philox_words((uint64_t)i, d, w);
+        float v[8];
+        if (left >= 8) {
+            load_vec<T, 8>(src, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < left ? load_one(src + e) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t u = e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+            v[e] = u >= d.threshold ? v[e] * d.scale : 0.f;
+        }
+        if (left >= 8) {
+            store_vec<T, 8>(dst, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) store_one(dst + e, v[e]);
+        }
+    }
+}
+
+__global__ void dropout_state_next_kernel(int64_t *state, int64_t calls, int64_t *used) {
+    const int64_t seed = state[0], offset = state[1];
+    used[0] = seed;
+    used[1] = offset;
+    state[1] = (int64_t)((uint64_t)offset + (uint64_t)calls);
+}
+
+// Sums of the partial rows, column by column in a fixed order: 16 columns x 64 slices of the rows per workgroup (the
+// columns are few, so narrow workgroups are what makes enough of them).
+__global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restrict__ partial, int blocks, int f,
+                                                            float *__restrict__ dweight, float *__restrict__ dbias) {
+    __shared__ float red[64][16];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int c = blockIdx.x * 16 + tx;
+    float s = 0.f;
+    if (c < 2 * f)
+        for (int b = ty; b < blocks; b += 64) s += partial[(int64_t)b * 2 * f + c];
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < 2 * f) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s += red[i][tx];
+        if (c < f) {
+            if (dweight) dweight[c] = s;
+        } else if (dbias) {
+            dbias[c - f] = s;
+        }
+    }
+}
+
+bool known_type(int t) { return t == ROF_F32 || t == ROF_BF16; }
+int size_of(int t) { return t == ROF_F32 ? 4 : 2; }
+bool aligned(const void *p, int size) { return ((uintptr_t)p) % (uintptr_t)size == 0; }
+
+// The threshold of a rate, or -1: the rate is taken to the nearest multiple of 2^-16.
+int drop_threshold(const rof_dropout_opts *d) {
+    if (!(d->p >= 0.0 && d->p <= 1.0)) return -1;
+    const int t = (int)(d->p * 65536.0 + 0.5);
+    if (t > 0 && (!d->state || !aligned(d->state, 8))) return -1;
+    return t;
+}
+float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.f; }
+
+NormShape norm_shape(int f, int x_dtype) {
+    const int vecs = (f * size_of(x_dtype) + 15) / 16;
+    NormShape s;
+    s.lpr = 64;
+    s.waves = vecs <= 256 ? 1 : vecs <= 1024 ? 4 : 16;
+    s.k = (vecs + s.lpr * s.waves - 1) / (s.lpr * s.waves);
+    s.rows = (s.waves > 4 ? s.waves * 64 : 256) / (s.lpr * s.waves);
+    return s;
+}
+
+int blocks_for(int64_t n, const NormShape &s, int most) {
+    return (int)std::min<int64_t>((n + s.rows - 1) / s.rows, s.waves > 4 ? most / 4 : most);
+}
+
+int launch_norm(const NormArgs &a, int x_dtype, int y_dtype, bool backward, const NormShape &s, int blocks, hipStream_t st) {
+    if (x_dtype == ROF_F32)
+        return y_dtype == ROF_F32 ? launch_norm_f32_f32(a, backward, s, blocks, st) : launch_norm_f32_bf16(a, backward, s, blocks, st);
+    return y_dtype == ROF_F32 ? launch_norm_bf16_f32(a, backward, s, blocks, st) : launch_norm_bf16_bf16(a, backward, s, blocks, st);
+}
+
+// the arguments that the two directions share
+int norm_args(NormArgs &a, const void *x, int x_dtype, int64_t ldx, int64_t n, int f, const float *weight, const float *bias,
+              double eps, int relu, const rof_dropout_opts *dropout, int y_dtype) {
+    if (n < 0 || f < 1 || ldx < f || (n && !x) || !(eps >= 0.0 && eps <= 1e30)) return ROF_ERR_ARG;
+    if (!known_type(x_dtype) || !known_type(y_dtype) || f > kMaxNormColumns) return ROF_ERR_UNSUPPORTED;
+    if (!aligned(x, size_of(x_dtype)) || !aligned(weight, 4) || !aligned(bias, 4)) return ROF_ERR_ARG;
+    a = NormArgs();
+    a.x = x;
+    a.ldx = ldx;
+    a.n = n;
+    a.f = f;
+    a.weight = weight;
+    a.bias = bias;
+    a.eps = eps;
+    a.relu = relu != 0;
+    a.scale = 1.f;
+    if (dropout) {
+        const int t = drop_threshold(dropout);
+        if (t < 0) return ROF_ERR_ARG;
+        a.drop = t > 0;
+        a.threshold = (uint32_t)t;
+        a.scale = drop_scale(t);
+        a.state = t > 0 ? dropout->state : nullptr;
+        a.call = dropout->call;
+    }
+    return ROF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rof_dropout_state_next(int64_t *state, int64_t calls, int64_t *used, void *stream) {
+    if (!state || !used || state == used || calls < 0 || !aligned(state, 8) || !aligned(used, 8)) return ROF_ERR_ARG;
+    hipLaunchKernelGGL(dropout_state_next_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, state, calls, used);
+    HIP_TRY(hipGetLastError());
+    return ROF_OK;
+}
+
+int rof_dropout(const void *x, int dtype, int64_t ldx, int64_t n, int f, void *out, int64_t ldo,
+                const rof_dropout_opts *dropout, void *stream) {
+    if (!dropout || n < 0 || f < 1 || ldx < f || ldo < f || (n && (!x || !out))) return ROF_ERR_ARG;
+    if (!known_type(dtype)) return ROF_ERR_UNSUPPORTED;
+    const int t = drop_threshold(dropout);
+    if (t < 0 || !aligned(x, size_of(dtype)) || !aligned(out, size_of(dtype))) return ROF_ERR_ARG;
+    if (n == 0) return ROF_OK;
+    DropoutArgs a;
+    a.x = x;
+    a.out = out;
+    a.ldx = ldx;
+    a.ldo = ldo;
+    a.f = f;
+    a.groups = (f + 7) / 8;
+    a.items = n * a.groups;
+    a.threshold = (uint32_t)t;
+    a.scale = drop_scale(t);
+    a.state = t > 0 ? dropout->state : nullptr;
+    a.call = dropout->call;
+    const int blocks = (int)std::min<int64_t>((a.items + 255) / 256, kForwardBlocks);
+    if (dtype == ROF_F32)
+        hipLaunchKernelGGL(dropout_kernel<float>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(dropout_kernel<bf16_t>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+    HIP_TRY(hipGetLastError());
+    return ROF_OK;
+}
+
+int rof_layer_norm(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, const float *weight, const float *bias, double eps,
+                   int relu, const rof_dropout_opts *dropout, void *out, int out_dtype, int64_t ldo, void *stream) {
+    NormArgs a;
+    const int rc = norm_args(a, x, x_dtype, ldx, n, f, weight, bias, eps, relu, dropout, out_dtype);
+    if (rc) return rc;
+    if (ldo < f || (n && !out) || !aligned(out, size_of(out_dtype))) return ROF_ERR_ARG;
+    if (n == 0) return ROF_OK;
+    a.out = out;
+    a.ldo = ldo;
+    const NormShape s = norm_shape(f, x_dtype);
+    return launch_norm(a, x_dtype, out_dtype, false, s, blocks_for(n, s, kForwardBlocks), (hipStream_t)stream);
+}
+
+size_t rof_layer_norm_backward_workspace_bytes(int64_t n, int f) {
+    if (n <= 0 || f <= 0) return 0;
+    return (size_t)std::min<int64_t>(n, kBackwardBlocks) * 2 * (size_t)f * sizeof(float);
+}
+
+int rof_layer_norm_backward(const void *dout, int dout_dtype, int64_t ldd, const void *x, int x_dtype, int64_t ldx, int64_t n,
+                            int f, const float *weight, const float *bias, double eps, int relu, const rof_dropout_opts *dropout,
+                            void *dx, int64_t lddx, float *dweight, float *dbias, void *workspace, size_t workspace_bytes,
+                            void *stream) {
+    NormArgs a;
+    const int rc = norm_args(a, x, x_dtype, ldx, n, f, weight, bias, eps, relu, dropout, dout_dtype);
+    if (rc) return rc;
+    if (ldd < f || (n && !dout) || !aligned(dout, size_of(dout_dtype)) || (dx && (lddx < f || !aligned(dx, size_of(x_dtype)))) ||
+        !aligned(dweight, 4) || !aligned(dbias, 4))
+        return ROF_ERR_ARG;
+    const bool params = dweight || dbias;
+    if (params && n && (!workspace || !aligned(workspace, 16) || workspace_bytes < rof_layer_norm_backward_workspace_bytes(n, f)))
+        return ROF_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    const NormShape s = norm_shape(f, x_dtype);
+    const int blocks = blocks_for(n, s, kBackwardBlocks);
+    if (n && (params || dx)) {
+        a.dout = dout;
+        a.ldd = ldd;
+        a.out = dx;
+        a.ldo = lddx;
+        a.partial = params ? (float *)workspace : nullptr;
+        const int status = launch_norm(a, x_dtype, dout_dtype, true, s, blocks, st);
+        if (status) return status;
+    }
+    if (params) {
+        hipLaunchKernelGGL(norm_params_kernel, dim3((2 * f + 15) / 16), dim3(1024), 0, st, (const float *)workspace, blocks, f,
+                           dweight, dbias);
+        HIP_TRY(hipGetLastError());
+    }
+    return ROF_OK;
+}
+
+}  // extern "C"

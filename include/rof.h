@@ -298,6 +298,58 @@ size_t rof_column_sums_workspace_bytes(int64_t n, int f);
 int rof_column_sums(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, float *out, void *workspace,
                     size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Device side: what stands between two convolutions of a network.  (Upstream leaves it to ready-made modules:
+ * dropout on the input of every layer but the first, ROF_evaluation/ROF_main.py:192-200; no normalisation.)
+ * All matrices are row-major with one row per node: [n, f] with a row stride in elements of at least f, float32
+ * or bfloat16, starting on a boundary of their element type (ROF_ERR_ARG otherwise).  Outputs must not overlap
+ * inputs.  Every call only enqueues on its stream and allocates nothing, so it can be captured.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Dropout without a stored mask.  Element (r, c) is kept where u >= t and then multiplied by 65536 / (65536 - t);
+ * otherwise it becomes 0, whatever it was.  t = floor(65536 p + 1/2): the rate is p to the nearest multiple of 2^-16
+ * (so less than 2^-17 is no dropout).  u is 16 bits of Philox4x32 with seven rounds under the key `seed`: the
+ * counter's low half is r * ceil(f / 8) + c / 8, its high half offset + call (mod 2^64), and field c % 8 of its four
+ * words (the low half of a word first) belongs to the element.  The mask thus depends on the row, the column, f,
+ * the seed and the offset only, not on the type, the strides or the launch.
+ * state: device int64[2] = {seed, offset}, read when the kernel runs (8-byte aligned; needed unless t = 0).  The
+ * backward pass has to be given the same values again. */
+typedef struct {
+    double p;               /* 0 ... 1 */
+    const int64_t *state;
+    int64_t call;           /* tells the calls of one step apart that share a state */
+} rof_dropout_opts;
+
+/* out = dropout(x); applied to the gradient of its output, with the same options, it is its own backward pass. */
+int rof_dropout(const void *x, int dtype, int64_t ldx, int64_t n, int f, void *out, int64_t ldo,
+                const rof_dropout_opts *dropout, void *stream);
+
+/* used[0..1] = state[0..1], then state[1] += calls: the values for one step (of at most `calls` calls, numbered from
+ * 0), which stay as they are until that step's backward pass is done, and a state that is ready for the next one.
+ * One launch, in stream order: a captured graph draws new masks at every replay. */
+int rof_dropout_state_next(int64_t *state, int64_t calls, int64_t *used, void *stream);
+
+/* Layer norm of every row, with the rest of a hidden layer in the same pass:
+ *     out = dropout(relu(h * weight + bias)),   h = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)
+ * weight, bias: device float32[f], or NULL for 1 and 0.  relu = 0 and dropout = NULL leave those out.  Statistics are
+ * float32 over the row as read; `out` is rounded once.  At most ROF_LAYER_NORM_MAX_COLUMNS columns
+ * (ROF_ERR_UNSUPPORTED otherwise: a row is kept in one workgroup's registers). */
+#define ROF_LAYER_NORM_MAX_COLUMNS 16384
+int rof_layer_norm(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, const float *weight, const float *bias,
+                   double eps, int relu, const rof_dropout_opts *dropout, void *out, int out_dtype, int64_t ldo,
+                   void *stream);
+
+/* Its gradient, from x and the gradient `dout` of `out` (of out's type): dx (of x's type), dweight and dbias
+ * (float32[f]); each may be NULL if it is not wanted.  weight, bias, eps, relu and dropout as in the forward call.
+ * Everything else is computed again from x; the ReLU's gate is decided in 64 bits where 32 do not settle its sign.
+ * Sums over rows have a fixed order (bitwise repeatable).  workspace: rof_layer_norm_backward_workspace_bytes(n, f)
+ * bytes, 16-byte aligned, needed when dweight or dbias is wanted; one per call in flight. */
+size_t rof_layer_norm_backward_workspace_bytes(int64_t n, int f);
+int rof_layer_norm_backward(const void *dout, int dout_dtype, int64_t ldd, const void *x, int x_dtype, int64_t ldx,
+                            int64_t n, int f, const float *weight, const float *bias, double eps, int relu,
+                            const rof_dropout_opts *dropout, void *dx, int64_t lddx, float *dweight, float *dbias,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
