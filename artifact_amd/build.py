@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,8 +22,8 @@ LIB = os.path.join(HERE, "librof.so")
 
 HOST_SOURCES = ["plan_builder.cpp", "hub_patterns.cpp", "dynamic_greedy.cpp", "layout.cpp"]
 HIP_SOURCES = ["agg_kernels.hip", "agg_rows_f32_partial.hip", "agg_rows_f32_dst.hip", "agg_cluster_f32.hip", "agg_coop_f32.hip", "agg_coop_bf16.hip",
-               "agg_rows_bf16_partial.hip", "agg_rows_bf16_dst.hip", "agg_cluster_bf16.hip", "row_ops.hip", "norm_f32_f32.hip",
-               "norm_f32_bf16.hip", "norm_bf16_f32.hip", "norm_bf16_bf16.hip"]
+               "agg_rows_bf16_partial.hip", "agg_rows_bf16_dst.hip", "agg_cluster_bf16.hip", "row_ops.hip"]
+HIP_SOURCES += [f"norm_{kind}_{x}_{y}.hip" for kind in ("bwd_relu", "bwd", "fwd") for x in ("f32", "bf16") for y in ("f32", "bf16")]
 
 # packed fp32 instructions stay off: the compiler must not form v_pk_{add,mul,fma}_f32
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
@@ -46,17 +47,26 @@ def build_library(verbose=True):
         o = os.path.join(objdir, s + ".o")
         _run([gxx] + HOST_FLAGS + inc + ["-c", os.path.join(CSRC, s), "-o", o])
         objs.append(o)
-    # the kernel translation units are independent: compile them side by side
-    procs = []
-    for s in HIP_SOURCES:
-        o = os.path.join(objdir, s + ".o")
-        cmd = [hipcc] + HIP_FLAGS + inc + ["-c", os.path.join(CSRC, s), "-o", o]
-        print("+", " ".join(cmd), flush=True)
-        procs.append((cmd, subprocess.Popen(cmd)))
-        objs.append(o)
-    for cmd, pr in procs:
-        if pr.wait() != 0:
-            raise subprocess.CalledProcessError(pr.returncode, cmd)
+    # the kernel translation units are independent: compile them side by side, as many as there are processors (a unit
+    # takes up to a gigabyte)
+    todo, running = list(HIP_SOURCES), []
+    objs += [os.path.join(objdir, s + ".o") for s in HIP_SOURCES]
+    try:
+        while todo or running:
+            while todo and len(running) < min(os.cpu_count() or 1, 16):
+                src = todo.pop(0)
+                cmd = [hipcc] + HIP_FLAGS + inc + ["-c", os.path.join(CSRC, src), "-o", os.path.join(objdir, src + ".o")]
+                print("+", " ".join(cmd), flush=True)
+                running.append((cmd, subprocess.Popen(cmd)))
+            for cmd, pr in list(running):
+                if pr.poll() is not None:
+                    running.remove((cmd, pr))
+                    if pr.returncode != 0:
+                        raise subprocess.CalledProcessError(pr.returncode, cmd)
+            time.sleep(0.05)
+    finally:
+        for _, pr in running:
+            pr.kill()
     _run([hipcc, "-shared", "-fPIC", "-o", LIB] + objs + ["-fopenmp", "-lgomp"])
     return LIB
 

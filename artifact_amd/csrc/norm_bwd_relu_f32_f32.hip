@@ -1,0 +1,10 @@
+// Layer-norm backward kernels with a ReLU for rows of type float whose normalised rows are of type float (see norm_rows.h).
+#include "norm_rows.h"
+
+namespace rofn {
+
+int norm_bwd_relu_f32_f32(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
+    return launch_norm_backward<float, float, true>(a, s, blocks, st);
+}
+
+}  // namespace rofn

@@ -1,0 +1,10 @@
+// Layer-norm forward kernels for rows of type bf16_t whose normalised rows are of type bf16_t (see norm_rows.h).
+#include "norm_rows.h"
+
+namespace rofn {
+
+int norm_fwd_bf16_bf16(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
+    return launch_norm_forward<bf16_t, bf16_t>(a, s, blocks, st);
+}
+
+}  // namespace rofn

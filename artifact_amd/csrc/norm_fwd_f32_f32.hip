@@ -1,0 +1,10 @@
+// Layer-norm forward kernels for rows of type float whose normalised rows are of type float (see norm_rows.h).
+#include "norm_rows.h"
+
+namespace rofn {
+
+int norm_fwd_f32_f32(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
+    return launch_norm_forward<float, float>(a, s, blocks, st);
+}
+
+}  // namespace rofn

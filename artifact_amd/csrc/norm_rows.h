@@ -1,5 +1,5 @@
 // Layer norm of feature rows, forward and backward, with the ReLU and the dropout that may follow it in the same pass.
-// Instantiated by norm_<input type>_<output type>.hip; the C ABI is in row_ops.hip.
+// Instantiated by norm_fwd_<input type>_<output type>.hip and norm_bwd_...; the C ABI is in row_ops.hip.
 //
 // Of each row x (f columns), with w and b the parameters:
 //     m = sum(x) / f      v = sum((x - m)^2) / f      r = 1 / sqrt(v + eps)      h = (x - m) r
@@ -16,7 +16,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "rof.h"
 #include "rof_internal.h"
@@ -79,98 +81,6 @@ __device__ __forceinline__ double group_sum(double v) {
     return v;
 }
 
-// ---- one row, spread over WAVES wavefronts of LPR lanes, K vectors of V columns per lane --------------------------
-// Vector j of lane l (0 .. LPR * WAVES - 1) covers the columns (j * LPR * WAVES + l) * V and the next V - 1, so that one
-// load instruction reads one contiguous piece of the row.  K is the least that covers f (checked by the launcher):
-// every vector but a lane's last is whole.
-template <typename TX, int LPR, int WAVES, int K>
-struct RowMap {
-    static constexpr int V = 16 / (int)sizeof(TX);
-    static constexpr int LANES = LPR * WAVES;
-    static constexpr int THREADS = WAVES > 4 ? WAVES * 64 : 256;
-    static constexpr int ROWS = THREADS / LANES;      // rows a workgroup works on at a time
-    static_assert(LPR == 64 || WAVES == 1, "a row is either part of a wavefront or whole wavefronts");
-
-    int l;         // lane within the row
-    int slot;      // which of the workgroup's rows
-    int last;      // columns of the last vector that exist (0 .. V)
-
-    __device__ __forceinline__ explicit RowMap(int f) {
-        l = (int)threadIdx.x % LANES;
-        slot = (int)threadIdx.x / LANES;
-        const int left = f - col(K - 1);
-        last = left < 0 ? 0 : left > V ? V : left;
-    }
-    __device__ __forceinline__ int col(int j) const { return (j * LANES + l) * V; }
-    __device__ __forceinline__ bool has(int j, int e) const { return j < K - 1 || e < last; }
-
-    // columns that do not exist read as zero, and so does everything when !ok
-    template <typename T>
-    __device__ __forceinline__ void load(const T *row, bool ok, float (&v)[K][V]) const {
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[j][e] = 0.f;
-            if (!ok) continue;
-            if (j < K - 1 || last == V) {
-                load_vec<T, V>(row + col(j), v[j]);
-            } else if (last > 0) {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (e < last) v[j][e] = load_one(row + col(j) + e);
-            }
-        }
-    }
-    template <typename T>
-    __device__ __forceinline__ void store(T *row, const float (&v)[K][V]) const {
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (j < K - 1 || last == V) {
-                store_vec<T, V>(row + col(j), v[j]);
-            } else if (last > 0) {
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (e < last) store_one(row + col(j) + e, v[j][e]);
-            }
-        }
-    }
-
-    // Sum over the row's lanes.  Of several wavefronts: through `part`, which holds two sets of WAVES numbers and is used
-    // alternately (`turn`), so that one barrier per sum is enough: a set is written again only after every wavefront has
-    // passed the next sum's barrier, that is, has read it.
-    template <typename S>
-    __device__ __forceinline__ S sum(S v, S (*part)[WAVES], int &turn) const {
-        v = group_sum<LPR>(v);
-        if constexpr (WAVES > 1) {
-            S *p = part[turn];
-            turn ^= 1;
-            if (l % 64 == 0) p[l / 64] = v;
-            __syncthreads();
-            v = S(0);
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) v += p[i];
-        }
-        return v;
-    }
-
-    // bit e of word j: whether the dropout keeps element (j, e).  A vector is a whole group of eight columns or half of one.
-    __device__ __forceinline__ void kept(const Drop &d, int64_t row, int f, uint32_t (&bits)[K]) const {
-        const uint64_t first = (uint64_t)row * (uint32_t)((f + 7) / 8);
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            uint32_t w[4];
-            philox_words(first + (uint32_t)(col(j) / 8), d, w);
-            bits[j] = 0;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const uint32_t word = V == 4 && (col(j) & 4) ? w[(2 + e / 2) % 4] : w[e / 2];
-                const uint32_t u = e % 2 ? word >> 16 : word & 0xffffu;
-                bits[j] |= (u >= d.threshold ? 1u : 0u) << e;
-            }
-        }
-    }
-};
-
 // s / f from the reciprocal, with what the product leaves of s added: a row of equal numbers (a node without in-edges under
 // a constant bias) has exactly that number as its mean, and no spread, where r = 1 / sqrt(eps) would magnify one rounding.
 __device__ __forceinline__ float mean_of(float s, float f, float inv_f) {
@@ -178,10 +88,274 @@ __device__ __forceinline__ float mean_of(float s, float f, float inv_f) {
     return fmaf(fmaf(-m, f, s), inv_f, m);
 }
 
+// ---- one row, spread over WAVES wavefronts of LPR lanes, K vectors of V columns per lane --------------------------
+// Vector j of lane l (0 .. LPR * WAVES - 1) covers the columns (j * LPR * WAVES + l) * V and the next V - 1, so that one
+// load instruction reads one contiguous piece of the row.  K is the least that covers f (checked by the launcher):
+// every vector but a lane's last is whole.
+template <typename TX, int LPR, int WAVES, int K>
+struct RowMap {
+    static constexpr int V = 16 / (int)sizeof(TX);
+    static constexpr int LANES = LPR * WAVES, WAVES_ = WAVES, K_ = K;
+    static constexpr int THREADS = WAVES > 1 ? WAVES * 64 : 256;
+    static constexpr int ROWS = THREADS / LANES;      // rows a workgroup works on at a time
+    static_assert(LPR == 64 || WAVES == 1, "a row is either part of a wavefront or whole wavefronts");
+    static_assert(WAVES == 1 || ROWS == 1, "the sums of several wavefronts meet in LDS that is there once per workgroup");
+
+    int l;         // lane within the row
+    int slot;      // which of the workgroup's rows
+    int last;      // columns of the last vector that exist (0 .. V)
+    int tail;      // f % V: what `last` is in the one lane where it is neither 0 nor V
+    bool full;     // the row fills all lanes' vectors: nothing below has to ask which columns exist
+    int from;      // column at which the last vector is read
+    int back;      // how far before its own columns that is (V - tail; 0 in lanes with whole vectors)
+    float columns, inv_columns;   // of the lane's wavefront, and 1 / columns (0 if it has none)
+
+    __device__ __forceinline__ explicit RowMap(int f) {
+        l = (int)threadIdx.x % LANES;
+        slot = (int)threadIdx.x / LANES;
+        tail = f % V;
+        full = f == LANES * K * V;
+        const int left = f - col(K - 1);
+        last = left < 0 ? 0 : left > V ? V : left;
+        from = last == V ? col(K - 1) : f - V;
+        back = last > 0 ? V - last : 0;
+        columns = columns_of(f, l / 64);
+        inv_columns = columns > 0.f ? 1.0f / columns : 0.f;
+    }
+    // the columns that wavefront i of the row covers
+    static __device__ __forceinline__ float columns_of(int f, int i) {
+        const int left = f - ((K - 1) * LANES + i * 64) * V, most = 64 * V;
+        return (float)((K - 1) * most + (left < 0 ? 0 : left > most ? most : left));
+    }
+    __device__ __forceinline__ int col(int j) const { return (j * LANES + l) * V; }
+    __device__ __forceinline__ bool has(int j, int e) const { return j < K - 1 || e < last; }
+
+    // A lane's part of a row as it lies in memory.  Nothing is branched around: a load whose result meets another value at a
+    // join is waited for there, and the next row's could not stay under way.  So a lane without columns reads the row's last
+    // V, and so does the last vector of a row that is no multiple of V, which is shifted into place when it is unpacked
+    // (element by element, rows of 47 columns took 1.4 times as long as rows of 48, bfloat16 2.6 times).  Only a row shorter
+    // than one vector is read element by element.
+    template <typename T>
+    struct Part {
+        Packed<T, V> p[K];
+        template <bool STREAM>
+        __device__ __forceinline__ void load(const RowMap &m, const T *row) {
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j) p[j].template load<STREAM>(row + m.col(j));
+            if constexpr (LANES == 1)
+                p[K - 1].load_few(row, m.last);
+            else
+                p[K - 1].template load<STREAM>(row + m.from);
+        }
+        // Waits for the row here.  Placed before this row's stores: the counter that a load is waited for by is in order, so
+        // a wait after them would be one for the stores as well.
+        __device__ __forceinline__ void arrive() {
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int i = 0; i < Packed<T, V>::WORDS; ++i) asm volatile("" : "+v"(p[j].w[i]));
+        }
+        // columns that do not exist are anything
+        __device__ __forceinline__ void unpack(const RowMap &m, float (&v)[K][V]) {
+            if (LANES > 1 && m.tail) p[K - 1].shift(m.back);
+#pragma unroll
+            for (int j = 0; j < K; ++j) p[j].unpack(v[j]);
+        }
+    };
+    // a parameter's columns: `none` without a parameter, `missing` where there is no column
+    __device__ __forceinline__ void load_param(const float *q, float none, float missing, float (&v)[K][V]) const {
+        Part<float> t;
+        if (q) {
+            t.template load<false>(*this, q);
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; ++j) t.p[j].clear();
+        }
+        t.unpack(*this, v);
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (!q) v[j][e] = none;
+                if (!has(j, e)) v[j][e] = missing;
+            }
+    }
+    template <bool STREAM, typename T>
+    __device__ __forceinline__ void store(T *row, const float (&v)[K][V]) const {
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            Packed<T, V> p;
+            p.pack(v[j]);
+            if (j < K - 1 || last == V)
+                p.template store<STREAM>(row + col(j));
+            else if (last > 0)
+                p.store_part(row + col(j), tail);
+        }
+    }
+
+    // Two sums over the row's lanes.  Of several wavefronts: through `part`, which holds two sets and is used alternately
+    // (`turn`), so that one barrier is enough: a set is written again only after every wavefront has passed the next one's
+    // barrier, that is, has read it.
+    template <typename S>
+    __device__ __forceinline__ void sum2(S &v0, S &v1, S (*part)[WAVES][2], int &turn) const {
+        v0 = group_sum<LPR>(v0);
+        v1 = group_sum<LPR>(v1);
+        if constexpr (WAVES > 1) {
+            S(*p)[2] = part[turn];
+            turn ^= 1;
+            if (l % 64 == 0) {
+                p[l / 64][0] = v0;
+                p[l / 64][1] = v1;
+            }
+            __syncthreads();
+            v0 = v1 = S(0);
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                v0 += p[i][0];
+                v1 += p[i][1];
+            }
+        }
+    }
+
+    // Mean of a row's elements and the sum of the squares of their differences from it; v becomes the differences (0 where
+    // there is no column).  Of several wavefronts each takes its own columns' first, and the row's follow from theirs: the
+    // squares are theirs plus (columns) (their mean - the mean)^2, one barrier for both.
+    __device__ __forceinline__ void moments(float (&v)[K][V], float f, float inv_f, float (*part)[WAVES][2], int &turn, float &mean,
+                                            float &squares) const {
+        float s = 0.f;
+        if (!full) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[K - 1][e] = has(K - 1, e) ? v[K - 1][e] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += v[j][e];
+        s = group_sum<LPR>(s);
+        float own = WAVES > 1 ? mean_of(s, columns, inv_columns) : mean_of(s, f, inv_f), q = 0.f;   // columns: the wavefront's
+        subtract(v, own);
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) q = fmaf(v[j][e], v[j][e], q);
+        q = group_sum<LPR>(q);
+        if constexpr (WAVES > 1) {
+            float(*p)[2] = part[turn];
+            turn ^= 1;
+            if (l % 64 == 0) {
+                p[l / 64][0] = own;
+                p[l / 64][1] = q;
+            }
+            __syncthreads();
+            const float first = own;
+            s = q = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) s = fmaf(columns_of((int)f, i), p[i][0], s);
+            own = mean_of(s, f, inv_f);
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                const float d = p[i][0] - own;
+                q += fmaf(columns_of((int)f, i) * d, d, p[i][1]);
+            }
+            subtract(v, own - first);
+        }
+        mean = own;
+        squares = q;
+    }
+    __device__ __forceinline__ void subtract(float (&v)[K][V], float from) const {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] -= from;
+        if (!full) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[K - 1][e] = has(K - 1, e) ? v[K - 1][e] : 0.f;
+        }
+    }
+
+    // The elements of a vector that the dropout keeps; `group` is the row's first.  A vector is a whole group of eight columns
+    // or half of one.
+    __device__ __forceinline__ void kept(const Drop &d, uint64_t group, int j, bool (&keep)[V]) const {
+        uint32_t w[4];
+        philox_words(group + (uint32_t)(col(j) / 8), d, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) keep[e] = drop_keeps(V == 4 && (col(j) & 4) ? w[(2 + e / 2) % 4] : w[e / 2], e, d);
+    }
+};
+
+// Where a lane's row begins, from one round of the launch to the next; it stays on its last row when the next would be
+// behind the matrix.  `all` (the same in every lane): no lane of the workgroup is that far, which spares the choice.
+template <typename T>
+struct Cursor {
+    T *at;
+    int64_t stride;
+    __device__ __forceinline__ Cursor(T *base, int64_t ld, int64_t row, int64_t rows, int64_t step)
+        : at(base + (row < rows ? row : rows - 1) * ld), stride(step * ld) {}
+    __device__ __forceinline__ void advance(bool all, bool further) {
+        if (all)
+            at += stride;
+        else if (further)
+            at += stride;
+    }
+};
+
+__device__ __forceinline__ float relu_of(float v) { return __builtin_elementwise_maximum(v, 0.f); }   // a NaN stays one
+
 template <int WAVES>
 struct Scratch {
-    float part[2][WAVES];
-    double part64[2][WAVES];
+    float part[2][WAVES][2];
+    double part64[2][WAVES][2];
+};
+
+// A lane's columns of a parameter.  In registers where a row is part of a wavefront or a wavefront; in LDS where it is
+// several, because there a lane holds up to 32 columns, and it is registers (of the gradient's sums above all) that
+// bound the wavefronts in flight: 20011 rows of 4099 bfloat16 columns take the backward launch 180 us with them in registers,
+// 128 from LDS.  A lane reads back only what it wrote, 16 bytes at a time in lane order, so there is neither a barrier nor
+// a conflict.
+template <typename Map>
+struct Param {
+    static constexpr bool kLds = Map::WAVES_ > 1;
+    static constexpr int V = Map::V, K = Map::K_, Q = V / 4;
+    using Store = float4[kLds ? K * Q * Map::LANES : 1];
+    float v[kLds ? 1 : K][V];
+    float4 *lds;
+
+    __device__ __forceinline__ Param(const Map &m, const float *q, float none, float missing, Store &store, float &most,
+                                     float factor = 1.f) {
+        float t[K][V];
+        m.load_param(q, none, missing, t);
+        most = 0.f;
+        lds = store + (kLds ? m.l : 0);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (m.has(j, e)) most = fmaxf(most, fabsf(t[j][e]));
+                t[j][e] *= factor;
+                if (!kLds) v[j][e] = t[j][e];
+            }
+            if (kLds) {
+#pragma unroll
+                for (int i = 0; i < Q; ++i)
+                    lds[(j * Q + i) * Map::LANES] = make_float4(t[j][4 * i], t[j][4 * i + 1], t[j][4 * i + 2], t[j][4 * i + 3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(int j, float (&to)[V]) const {
+        if constexpr (kLds) {
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const float4 t = lds[(j * Q + i) * Map::LANES];
+                to[4 * i] = t.x;
+                to[4 * i + 1] = t.y;
+                to[4 * i + 2] = t.z;
+                to[4 * i + 3] = t.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) to[e] = v[j][e];
+        }
+    }
 };
 
 template <typename TX, typename TY, int LPR, int WAVES, int K>
@@ -191,188 +365,254 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
     __shared__ Scratch<WAVES> sh;
     const Map m(a.f);
     int turn = 0;
-    float w[K][V], b[K][V];
-    m.load(a.weight, a.weight != nullptr, w);
-    m.load(a.bias, a.bias != nullptr, b);
-    if (!a.weight) {
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) w[j][e] = 1.f;
-    }
+    __shared__ typename Param<Map>::Store wstore, bstore;
+    float most;
+    // the dropout's scale is in the parameters: it is positive, so it passes through the ReLU
+    const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, most, a.scale), bias(m, a.bias, 0.f, 0.f, bstore, most, a.scale);
     const Drop drop(a);
-    const float inv_f = 1.0f / (float)a.f;
-    for (int64_t base = (int64_t)blockIdx.x * Map::ROWS; base < a.n; base += (int64_t)gridDim.x * Map::ROWS) {
-        const int64_t row = base + m.slot;
-        const bool ok = row < a.n;
+    const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
+    const int64_t step = a.step, first = (int64_t)blockIdx.x * a.chunk, stop = std::min(a.n, first + a.span);
+    const uint32_t groups = (uint32_t)(a.f + 7) / 8;
+    typename Map::template Part<TX> next;
+    const int64_t row = first + m.slot;
+    uint64_t group = (uint64_t)row * groups;
+    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n, step);
+    Cursor<TY> out((TY *)a.out, a.ldo, row, a.n, step);
+    next.template load<false>(m, x.at);
+    for (int64_t left = stop - first; left > 0; left -= step) {
+        const bool ok = m.slot < left, all = step + Map::ROWS <= left, further = m.slot + step < left;
         float v[K][V];
-        m.load((const TX *)a.x + row * a.ldx, ok, v);
-        float s = 0.f;
+        next.unpack(m, v);
+        x.advance(all, further);
+        next.template load<false>(m, x.at);   // on its way while this row is worked on
+        float mean, squares;
+        m.moments(v, f, inv_f, sh.part, turn, mean, squares);
+        const float r = rsqrtf(fmaf(squares, inv_f, eps));
 #pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += v[j][e];
-        const float mean = mean_of(m.sum(s, sh.part, turn), (float)a.f, inv_f);
-        s = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                v[j][e] = m.has(j, e) ? v[j][e] - mean : 0.f;
-                s = fmaf(v[j][e], v[j][e], s);
-            }
-        const float r = 1.0f / sqrtf(m.sum(s, sh.part, turn) * inv_f + (float)a.eps);
-        uint32_t bits[K];
-        if (a.drop) m.kept(drop, row, a.f, bits);
-#pragma unroll
-        for (int j = 0; j < K; ++j)
+        for (int j = 0; j < K; ++j) {
+            float w[V], b[V];
+            weight.get(j, w);
+            bias.get(j, b);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                float y = fmaf(v[j][e] * r, w[j][e], b[j][e]);
-                if (a.relu) y = y < 0.f ? 0.f : y;   // a NaN stays one
-                if (a.drop) y = (bits[j] >> e & 1u) ? y * drop.scale : 0.f;
-                v[j][e] = y;
+                v[j][e] = fmaf(v[j][e] * r, w[e], b[e]);
+                if (a.relu) v[j][e] = relu_of(v[j][e]);
             }
-        if (ok) m.store((TY *)a.out + row * a.ldo, v);
+            if (a.drop) {
+                bool keep[V];
+                m.kept(drop, group, j, keep);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[j][e] = keep[e] ? v[j][e] : 0.f;
+            }
+        }
+        next.arrive();
+        if (ok) m.template store<false>(out.at, v);
+        out.advance(all, further);
+        group += (uint64_t)step * groups;
     }
 }
 
 // The ReLU's gate decides whether a whole gradient passes, so its border must not move with the order in which a variant
 // of this kernel adds.  Where |pre| is within the rounding error that 32 bits can have there, the wavefront (or the
 // workgroup that shares the row) takes the row's statistics again in 64 bits and decides by those.  The bound, in half
-// steps u = 2^-24: a lane adds up to 32 numbers, the butterfly and the wavefronts 6 + 16 more, so m is off by q / r with
-// q = 55 u (|m| r + 1); h by q + 34 u |h| + |h| q^2 / 2, and the last operation adds 2 u (|h w| + |b|).  With |m| r up to
-// 2^10 the square is below q, and all of it below 128 u = 2^-17 times |w| (r (|x| + |m|) + 1) + |b|; a row whose mean is
-// further than that from zero is always decided in 64 bits.  About 2 elements in 10^5 are that close on normally
-// distributed rows.
+// steps u = 2^-24: a lane adds up to 32 numbers, the butterfly 6 more, the wavefronts' means are rounded and weighted (3) and
+// up to 16 of them added, so m is off by q / r with q = 58 u (|m| r + 1); h by q + 36 u |h| + |h| q^2 / 2, and the last
+// operation adds 2 u (|h w| + |b|).  Near the border |h w| is |b|, and for |m| r up to 2^10 q^2 / 2 is below 100 u, so all
+// of it is below 128 u = 2^-17 times |w| (2 |m| r + 1) + 2 |b|; for w and b a lane's largest serve, so that the common path
+// has one minimum per element.  A row whose mean is further from zero is always decided in 64 bits.  About 4 elements in
+// 10^5 are that close on normally distributed rows.
 constexpr float kBorder = 7.62939453125e-06f;
 constexpr float kFarMean = 1024.f;
 
-template <typename TX, typename TY, int LPR, int WAVES, int K>
+// The exact sign of pre, in place of its value.  Rare, so it is kept small: it reads the row again.
+template <typename Map, typename TX>
+__device__ __forceinline__ void gate64(const Map &m, const NormArgs &a, const TX *row, bool ok, double (*part)[Map::WAVES_][2], int &turn,
+                                       float (&pre)[Map::K_][Map::V]) {
+    constexpr int V = Map::V, K = Map::K_;
+    auto at = [&](int j, float (&v)[V]) {
+        const int count = !ok ? 0 : j < K - 1 ? V : m.last;
+        Packed<TX, V> p;
+        p.load_few(row + m.col(j), count);
+        p.unpack(v);
+        return count;
+    };
+    float v[V];
+    double s = 0.0, none = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < K; ++j) {
+        at(j, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += (double)v[e];
+    }
+    m.sum2(s, none, part, turn);
+    const double mean = s / a.f;
+    s = none = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < K; ++j) {
+        const int count = at(j, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double c = e < count ? (double)v[e] - mean : 0.0;
+            s = fma(c, c, s);
+        }
+    }
+    m.sum2(s, none, part, turn);
+    const double r = 1.0 / sqrt(s / a.f + a.eps);
+    uint32_t gate = 0;
+#pragma unroll 1
+    for (int j = 0; j < K; ++j) {
+        const int count = at(j, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (e < count) {
+                const int c = m.col(j) + e;
+                const double w = a.weight ? (double)a.weight[c] : 1.0, b = a.bias ? (double)a.bias[c] : 0.0;
+                gate |= (fma(((double)v[e] - mean) * r, w, b) > 0.0 ? 1u : 0u) << (j * V + e);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) pre[j][e] = (gate >> (j * V + e) & 1u) ? 1.f : 0.f;
+}
+
+// nothing, where the bias is not needed (without a ReLU the gradient does not depend on it)
+struct NoParam {
+    using Store = float4[1];
+    template <typename Map>
+    __device__ __forceinline__ NoParam(const Map &, const float *, float, float, Store &, float &) {}
+};
+template <typename Map, bool NEEDED>
+using ParamOf = std::conditional_t<NEEDED, Param<Map>, NoParam>;
+
+template <typename TX, typename TY, int LPR, int WAVES, int K, bool RELU, bool STREAM>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd_kernel(NormArgs a) {
     using Map = RowMap<TX, LPR, WAVES, K>;
     constexpr int V = Map::V;
     __shared__ Scratch<WAVES> sh;
     const Map m(a.f);
     int turn = 0, turn64 = 0;
-    float w[K][V], b[K][V], dw[K][V], db[K][V];
-    m.load(a.weight, a.weight != nullptr, w);
-    m.load(a.bias, a.bias != nullptr && a.relu, b);
+    __shared__ typename Param<Map>::Store wstore;
+    __shared__ typename ParamOf<Map, RELU>::Store bstore;
+    float dw[K][V], db[K][V], wmost, bmost;
+    const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, wmost);
+    const ParamOf<Map, RELU> bias(m, a.bias, 0.f, 1.f, bstore, bmost);   // pre = 1 in columns that do not exist: never near the border
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.f;
+    const Drop drop(a);
+    const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
+    const int64_t step = a.step, first = (int64_t)blockIdx.x * a.chunk, stop = std::min(a.n, first + a.span);
+    const uint32_t groups = (uint32_t)(a.f + 7) / 8;
+    typename Map::template Part<TX> next_x;
+    typename Map::template Part<TY> next_d;
+    const int64_t row = first + m.slot;
+    uint64_t group = (uint64_t)row * groups;
+    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n, step);
+    Cursor<const TY> dout((const TY *)a.dout, a.ldd, row, a.n, step);
+    Cursor<TX> dx((TX *)a.out, a.ldo, row, a.n, step);
+    next_x.template load<STREAM>(m, x.at);
+    next_d.template load<STREAM>(m, dout.at);
+    for (int64_t left = stop - first; left > 0; left -= step) {
+        const bool ok = m.slot < left, all = step + Map::ROWS <= left, further = m.slot + step < left;
+        float h[K][V], d[K][V];
+        next_x.unpack(m, h);
+        next_d.unpack(m, d);
+        const TX *const here = x.at;
+        x.advance(all, further);   // on their way while this row is worked on
+        dout.advance(all, further);
+        next_x.template load<STREAM>(m, x.at);
+        next_d.template load<STREAM>(m, dout.at);
+        // (columns that do not exist hold other columns of d: their weight is 0, and their sums are not stored)
+        if (left < Map::ROWS) {   // lane groups behind the last row work on it once more and add nothing
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[j][e] = ok ? d[j][e] : 0.f;
+        }
+        float mean, squares;
+        m.moments(h, f, inv_f, sh.part, turn, mean, squares);
+        const float r = rsqrtf(fmaf(squares, inv_f, eps));
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[j][e] *= r;
+        if (a.drop) {   // its scale comes last: everything below is linear in d
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                bool keep[V];
+                m.kept(drop, group, j, keep);
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[j][e] = keep[e] ? d[j][e] : 0.f;
+            }
+        }
+        if constexpr (RELU) {
+            float pre[K][V], least = __builtin_inff();
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                float w[V], b[V];
+                weight.get(j, w);
+                bias.get(j, b);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    pre[j][e] = fmaf(h[j][e], w[e], b[e]);
+                    least = fminf(least, fabsf(pre[j][e]));
+                }
+            }
+            const float far = r * fabsf(mean);
+            const bool close = ok && (far > kFarMean || least <= kBorder * fmaf(fmaf(2.f, far, 1.f), wmost, 2.f * bmost));
+            if (WAVES > 1 ? __syncthreads_or(close) : __any(close)) gate64(m, a, here, ok, sh.part64, turn64, pre);
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[j][e] = pre[j][e] > 0.f ? d[j][e] : 0.f;
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            float w[V];
+            weight.get(j, w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                dw[j][e] = fmaf(d[j][e], h[j][e], dw[j][e]);
+                db[j][e] += d[j][e];
+                d[j][e] *= w[e];
+                s1 += d[j][e];
+                s2 = fmaf(d[j][e], h[j][e], s2);
+            }
+        }
+        m.sum2(s1, s2, sh.part, turn);
+        next_x.arrive();
+        next_d.arrive();
+        if (a.out) {
+            const float rs = r * a.scale;
+            s1 *= -inv_f * rs;
+            s2 *= -inv_f * rs;
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[j][e] = fmaf(h[j][e], s2, fmaf(d[j][e], rs, s1));
+            if (ok) m.template store<STREAM>(dx.at, d);
+            dx.advance(all, further);
+        }
+        group += (uint64_t)step * groups;
+    }
+    if (!a.partial) return;
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            if (!a.weight) w[j][e] = 1.f;
-            dw[j][e] = db[j][e] = 0.f;
+            dw[j][e] *= a.scale;
+            db[j][e] *= a.scale;
         }
-    const Drop drop(a);
-    const float inv_f = 1.0f / (float)a.f;
-    for (int64_t base = (int64_t)blockIdx.x * Map::ROWS; base < a.n; base += (int64_t)gridDim.x * Map::ROWS) {
-        const int64_t row = base + m.slot;
-        const bool ok = row < a.n;
-        float x[K][V], d[K][V];
-        m.load((const TX *)a.x + row * a.ldx, ok, x);
-        m.load((const TY *)a.dout + row * a.ldd, ok, d);
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += x[j][e];
-        const float mean = mean_of(m.sum(s, sh.part, turn), (float)a.f, inv_f);
-        s = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float c = m.has(j, e) ? x[j][e] - mean : 0.f;
-                s = fmaf(c, c, s);
-            }
-        const float r = 1.0f / sqrtf(m.sum(s, sh.part, turn) * inv_f + (float)a.eps);
-        if (a.drop || a.relu) {
-            uint32_t bits[K];   // the elements whose gradient passes
-#pragma unroll
-            for (int j = 0; j < K; ++j) bits[j] = 0xffu;
-            if (a.drop) m.kept(drop, row, a.f, bits);
-            if (a.relu) {
-                uint32_t gate[K];
-                bool near = r * fabsf(mean) > kFarMean;
-#pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    gate[j] = 0;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float pre = fmaf((x[j][e] - mean) * r, w[j][e], b[j][e]);
-                        const float most = fmaf(fabsf(w[j][e]), fmaf(r, fabsf(x[j][e]) + fabsf(mean), 1.f), fabsf(b[j][e]));
-                        near |= m.has(j, e) && (bits[j] >> e & 1u) && fabsf(pre) <= kBorder * most;
-                        gate[j] |= (pre > 0.f ? 1u : 0u) << e;
-                    }
-                }
-                near = near && ok;
-                if (WAVES > 1 ? __syncthreads_or(near) : __any(near)) {
-                    double s64 = 0.0;
-#pragma unroll
-                    for (int j = 0; j < K; ++j)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) s64 += (double)x[j][e];
-                    const double m64 = m.sum(s64, sh.part64, turn64) / a.f;
-                    s64 = 0.0;
-#pragma unroll
-                    for (int j = 0; j < K; ++j)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const double c = m.has(j, e) ? (double)x[j][e] - m64 : 0.0;
-                            s64 = fma(c, c, s64);
-                        }
-                    const double r64 = 1.0 / sqrt(m.sum(s64, sh.part64, turn64) / a.f + a.eps);
-#pragma unroll
-                    for (int j = 0; j < K; ++j) {
-                        gate[j] = 0;
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const double h = ((double)x[j][e] - m64) * r64;
-                            gate[j] |= (fma(h, (double)w[j][e], (double)b[j][e]) > 0.0 ? 1u : 0u) << e;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < K; ++j) bits[j] &= gate[j];
-            }
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) d[j][e] = (bits[j] >> e & 1u) ? d[j][e] * drop.scale : 0.f;
-        }
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float h = m.has(j, e) ? (x[j][e] - mean) * r : 0.f;
-                dw[j][e] = fmaf(d[j][e], h, dw[j][e]);
-                db[j][e] += d[j][e];
-                const float g = d[j][e] * w[j][e];
-                s1 += g;
-                s2 = fmaf(g, h, s2);
-                x[j][e] = h;
-                d[j][e] = g;
-            }
-        s1 = m.sum(s1, sh.part, turn) * inv_f;
-        s2 = m.sum(s2, sh.part, turn) * inv_f;
-        if (a.out) {
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-                for (int e = 0; e < V; ++e) d[j][e] = r * (d[j][e] - s1 - x[j][e] * s2);
-            if (ok) m.store((TX *)a.out + row * a.ldo, d);
-        }
-    }
-    if (!a.partial) return;
     // The workgroup's sums, as one row of 2 f floats: lane groups of a wavefront first, then the wavefronts one after the
     // other through LDS (a fixed order).
     float *const pw = a.partial + (int64_t)blockIdx.x * 2 * a.f, *const pb = pw + a.f;
     if constexpr (WAVES > 1) {
-        m.store(pw, dw);
-        m.store(pb, db);
+        m.template store<false>(pw, dw);
+        m.template store<false>(pb, db);
     } else {
         __shared__ float red[2 * LPR * K * V];
 #pragma unroll
@@ -405,35 +645,50 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 }
 
 // ---- launch ---------------------------------------------------------------------------------------------------------
-template <typename TX, typename TY, int LPR, int WAVES, int K>
-int launch_variant(const NormArgs &a, bool backward, int blocks, hipStream_t st) {
-    using Map = RowMap<TX, LPR, WAVES, K>;
-    if (backward)
-        hipLaunchKernelGGL((norm_bwd_kernel<TX, TY, LPR, WAVES, K>), dim3(blocks), dim3(Map::THREADS), 0, st, a);
-    else
-        hipLaunchKernelGGL((norm_fwd_kernel<TX, TY, LPR, WAVES, K>), dim3(blocks), dim3(Map::THREADS), 0, st, a);
-    HIP_TRY(hipGetLastError());
-    return ROF_OK;
+// The variants that norm_shape (row_ops.hip) chooses among: lanes of a wavefront, wavefronts and vectors per lane.
+// (V(lanes, wavefronts, vectors); STREAMED: those that also exist with streaming accesses.)
+#define ROF_NORM_STREAMED(V) V(8, 1, 1) V(16, 1, 1) V(32, 1, 1) V(64, 1, 1) V(64, 1, 2) V(64, 2, 2) V(64, 4, 2) V(64, 8, 2)
+#define ROF_NORM_OTHERS(V) V(1, 1, 1) V(2, 1, 1) V(4, 1, 1) V(64, 1, 3) V(64, 4, 3) V(64, 8, 3) V(64, 8, 4)
+#define ROF_NORM_F32_ONLY(V) V(64, 16, 3) V(64, 16, 4)   // 16384 bfloat16 columns are 2048 vectors
+
+template <typename TX, typename TY>
+int launch_norm_forward(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
+#define ROF_NORM_LAUNCH(LPR, WAVES, K)                                                                                          \
+    if (s.lpr == LPR && s.waves == WAVES && s.k == K) {                                                                         \
+        hipLaunchKernelGGL((norm_fwd_kernel<TX, TY, LPR, WAVES, K>), dim3(blocks), dim3((RowMap<TX, LPR, WAVES, K>::THREADS)), 0, \
+                           st, a);                                                                                              \
+        HIP_TRY(hipGetLastError());                                                                                             \
+        return ROF_OK;                                                                                                          \
+    }
+    ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
+    ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
+    if constexpr (sizeof(TX) == 4) {
+        ROF_NORM_F32_ONLY(ROF_NORM_LAUNCH)
+    }
+#undef ROF_NORM_LAUNCH
+    return ROF_ERR_UNSUPPORTED;
 }
 
-// the variants that norm_shape (row_ops.hip) chooses among
-template <typename TX, typename TY>
-int launch_norm(const NormArgs &a, bool backward, const NormShape &s, int blocks, hipStream_t st) {
-#define ROF_NORM_VARIANT(LPR, WAVES, K) \
-    if (s.lpr == LPR && s.waves == WAVES && s.k == K) return launch_variant<TX, TY, LPR, WAVES, K>(a, backward, blocks, st)
-    ROF_NORM_VARIANT(64, 1, 1);
-    ROF_NORM_VARIANT(64, 1, 2);
-    ROF_NORM_VARIANT(64, 1, 3);
-    ROF_NORM_VARIANT(64, 1, 4);
-    ROF_NORM_VARIANT(64, 4, 2);
-    ROF_NORM_VARIANT(64, 4, 3);
-    ROF_NORM_VARIANT(64, 4, 4);
-    ROF_NORM_VARIANT(64, 16, 2);
-    if constexpr (sizeof(TX) == 4) {   // 16384 bfloat16 columns are 2048 vectors
-        ROF_NORM_VARIANT(64, 16, 3);
-        ROF_NORM_VARIANT(64, 16, 4);
+template <typename TX, typename TY, bool RELU>
+int launch_norm_backward(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
+#define ROF_NORM_LAUNCH_AS(LPR, WAVES, K, STREAM)                                                                               \
+    if (s.lpr == LPR && s.waves == WAVES && s.k == K && s.stream == STREAM) {                                                   \
+        hipLaunchKernelGGL((norm_bwd_kernel<TX, TY, LPR, WAVES, K, RELU, STREAM>), dim3(blocks),                                \
+                           dim3((RowMap<TX, LPR, WAVES, K>::THREADS)), 0, st, a);                                               \
+        HIP_TRY(hipGetLastError());                                                                                             \
+        return ROF_OK;                                                                                                          \
     }
-#undef ROF_NORM_VARIANT
+#define ROF_NORM_LAUNCH(LPR, WAVES, K) ROF_NORM_LAUNCH_AS(LPR, WAVES, K, false)
+#define ROF_NORM_LAUNCH_STREAMED(LPR, WAVES, K) ROF_NORM_LAUNCH_AS(LPR, WAVES, K, true)
+    ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
+    ROF_NORM_STREAMED(ROF_NORM_LAUNCH_STREAMED)
+    ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
+    if constexpr (sizeof(TX) == 4) {
+        ROF_NORM_F32_ONLY(ROF_NORM_LAUNCH)
+    }
+#undef ROF_NORM_LAUNCH_STREAMED
+#undef ROF_NORM_LAUNCH
+#undef ROF_NORM_LAUNCH_AS
     return ROF_ERR_UNSUPPORTED;
 }
 

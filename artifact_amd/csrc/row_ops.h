@@ -19,6 +19,7 @@ struct NormArgs {
     float *partial;          // backward: [workgroups][2][f], or null
     int64_t ldx, ldd, ldo;
     int64_t n;
+    int64_t chunk, step, span;   // workgroup i works on the rows i chunk ... + span, `step` of them apart from one round to the next
     int32_t f;
     int32_t relu;
     int32_t drop;            // dropout on
@@ -29,25 +30,29 @@ struct NormArgs {
     double eps;
 };
 
-// lanes of a row, vectors per lane: the variant of the layer-norm kernels that covers f columns
+// the variant of the layer-norm kernels for a width, see norm_shape
 struct NormShape {
-    int lpr, waves, k;
-    int rows;                // rows a workgroup works on at a time
+    int lpr, waves, k;       // lanes of a wavefront and wavefronts that share a row, vectors per lane
+    bool stream;             // backward: streaming accesses
+    int rows() const { return waves > 1 ? 1 : 256 / lpr; }   // that a workgroup works on at a time
 };
 
-int launch_norm_f32_f32(const NormArgs &a, bool backward, const NormShape &s, int blocks, hipStream_t st);
-int launch_norm_f32_bf16(const NormArgs &a, bool backward, const NormShape &s, int blocks, hipStream_t st);
-int launch_norm_bf16_f32(const NormArgs &a, bool backward, const NormShape &s, int blocks, hipStream_t st);
-int launch_norm_bf16_bf16(const NormArgs &a, bool backward, const NormShape &s, int blocks, hipStream_t st);
+#define ROF_NORM_TYPES(V) V(f32_f32) V(f32_bf16) V(bf16_f32) V(bf16_bf16)
+#define ROF_NORM_DECLARE(T)                                                                          \
+    int norm_fwd_##T(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st);             \
+    int norm_bwd_##T(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st);             \
+    int norm_bwd_relu_##T(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st);
+ROF_NORM_TYPES(ROF_NORM_DECLARE)
+#undef ROF_NORM_DECLARE
 
 #if defined(__HIPCC__)
 // The dropout of one launch: key and offset are read from the device, so a captured launch draws from whatever the state
 // holds when it is replayed.
 struct Drop {
-    uint32_t k0 = 0, k1 = 0, o0 = 0, o1 = 0, threshold;
-    float scale;
+    uint32_t k0 = 0, k1 = 0, o0 = 0, o1 = 0;
+    uint32_t last;           // the largest 16-bit number that drops an element: threshold - 1
     template <typename Args>
-    __device__ __forceinline__ explicit Drop(const Args &a) : threshold(a.threshold), scale(a.scale) {
+    __device__ __forceinline__ explicit Drop(const Args &a) : last(a.threshold - 1) {
         if (a.state) {
             const uint64_t seed = (uint64_t)a.state[0], offset = (uint64_t)a.state[1] + (uint64_t)a.call;
             k0 = (uint32_t)seed;
@@ -57,6 +62,12 @@ struct Drop {
         }
     }
 };
+
+// Whether the element of field e (0 .. 7) is kept.  One comparison each: 16 bits of the low half of a word, 32 bits for the
+// high half, whose lower bits cannot change the outcome against a bound that ends in ones.
+__device__ __forceinline__ bool drop_keeps(uint32_t word, int e, const Drop &d) {
+    return e % 2 ? word > (d.last << 16 | 0xffffu) : (uint16_t)word > (uint16_t)d.last;
+}
 
 // Philox4x32 with seven rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011: the
 // least that passes BigCrush): the four words of the counter (group, offset) under the key.  A group is eight columns of
@@ -80,82 +91,111 @@ __device__ __forceinline__ void philox_words(uint64_t group, const Drop &d, uint
     w[3] = c3;
 }
 
-// Rows start wherever their type's alignment allows (packed rows of 47 columns): the vectors promise no more than that,
-// and gfx950 reads and writes them with one instruction all the same.
-typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u4_t __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u2_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float load_one(const float *p) { return *p; }
-__device__ __forceinline__ float load_one(const bf16_t *p) { return __uint_as_float((uint32_t)*p << 16); }
 // rounded to nearest even, like every bfloat16 this library stores
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     const f2_t v = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2_t));
 }
-__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
-__device__ __forceinline__ void store_one(bf16_t *p, float v) { *p = (bf16_t)bf16_pair(v, 0.f); }
-
+// V elements of a row as they lie in memory, so that a row can be under way in as few registers as it has bytes.
+// Rows start wherever their type's alignment allows (packed rows of 47 columns), and the accesses promise no more than
+// that: gfx950 reads and writes 4, 8, 12 and 16 bytes at any address, each with one instruction.
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T *p, float (&v)[V]) {
-    if constexpr (sizeof(T) == 4) {
+struct Packed {
+    static constexpr int WORDS = V * (int)sizeof(T) / 4, PIECE = WORDS < 4 ? WORDS : 4;
+    typedef uint32_t piece_t __attribute__((ext_vector_type(PIECE), aligned(sizeof(T))));
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f4_t t = *reinterpret_cast<const f4_t *>(p + i);
-            v[i] = t.x;
-            v[i + 1] = t.y;
-            v[i + 2] = t.z;
-            v[i + 3] = t.w;
+        for (int i = 0; i < WORDS; ++i) w[i] = 0;
+    }
+    // STREAM: bypassing the caches' replacement, for matrices that they do not hold until somebody reads them again
+    template <bool STREAM = false>
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += PIECE) {
+            const piece_t *at = reinterpret_cast<const piece_t *>(p) + i / PIECE;
+            const piece_t t = STREAM ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k) w[i + k] = t[k];
         }
-    } else {
-        uint32_t t[V / 2];
-        if constexpr (V == 8) {
-            const u4_t u = *reinterpret_cast<const u4_t *>(p);
-            t[0] = u.x;
-            t[1] = u.y;
-            t[2] = u.z;
-            t[3] = u.w;
+    }
+    template <bool STREAM = false>
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += PIECE) {
+            piece_t t;
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k) t[k] = w[i + k];
+            piece_t *at = reinterpret_cast<piece_t *>(p) + i / PIECE;
+            if (STREAM)
+                __builtin_nontemporal_store(t, at);
+            else
+                *at = t;
+        }
+    }
+    // Moves the elements `by` (less than V) places to the front; what comes in behind them is anything.
+    __device__ __forceinline__ void shift(int by) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t bytes = (uint32_t)(by & 1) * 2;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = __builtin_amdgcn_alignbyte(w[i + 1 < WORDS ? i + 1 : i], w[i], bytes);
+            by >>= 1;
+        }
+        shift_words<1>(by);
+        shift_words<2>(by);
+        shift_words<4>(by);
+    }
+    // The first `count` elements only, the others zero (a row shorter than a vector; no hot path).
+    __device__ __forceinline__ void load_few(const T *p, int count) {
+        clear();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (e < count) {
+                T t;
+                __builtin_memcpy(&t, p + e, sizeof(T));
+                if constexpr (sizeof(T) == 4)
+                    w[e] = __float_as_uint(t);
+                else
+                    w[e / 2] |= (uint32_t)t << (e % 2 * 16);
+            }
+        }
+    }
+    // The first `count` (less than V) elements only.  `count` is the same for the whole launch, so the choice among the
+    // V - 1 sizes is a scalar branch, and a size is one or two instructions.
+    template <int C = V - 1>
+    __device__ __forceinline__ void store_part(T *p, int count) const {
+        if (count == C)
+            __builtin_memcpy(p, w, C * sizeof(T));
+        else if constexpr (C > 1)
+            store_part<C - 1>(p, count);
+    }
+    template <int STEP>
+    __device__ __forceinline__ void shift_words(int by) {
+#pragma unroll
+        for (int i = 0; i + STEP < WORDS; ++i) {
+            const uint32_t here = w[i], there = w[i + STEP];   // as values: a choice between addresses would need memory
+            w[i] = (by & STEP) ? there : here;
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&v)[V]) const {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            v[e] = __uint_as_float(sizeof(T) == 4 ? w[e] : e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+    __device__ __forceinline__ void pack(const float (&v)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = __float_as_uint(v[e]);
         } else {
-            const u2_t u = *reinterpret_cast<const u2_t *>(p);
-            t[0] = u.x;
-            t[1] = u.y;
-        }
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            v[2 * i] = __uint_as_float(t[i] << 16);
-            v[2 * i + 1] = __uint_as_float(t[i] & 0xffff0000u);
+            for (int e = 0; e < V; e += 2) w[e / 2] = bf16_pair(v[e], v[e + 1]);
         }
     }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(T *p, const float (&v)[V]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            f4_t t;
-            t.x = v[i];
-            t.y = v[i + 1];
-            t.z = v[i + 2];
-            t.w = v[i + 3];
-            *reinterpret_cast<f4_t *>(p + i) = t;
-        }
-    } else if constexpr (V == 8) {
-        u4_t t;
-        t.x = bf16_pair(v[0], v[1]);
-        t.y = bf16_pair(v[2], v[3]);
-        t.z = bf16_pair(v[4], v[5]);
-        t.w = bf16_pair(v[6], v[7]);
-        *reinterpret_cast<u4_t *>(p) = t;
-    } else {
-        u2_t t;
-        t.x = bf16_pair(v[0], v[1]);
-        t.y = bf16_pair(v[2], v[3]);
-        *reinterpret_cast<u2_t *>(p) = t;
-    }
-}
+};
 #endif
 
 }  // namespace rofn

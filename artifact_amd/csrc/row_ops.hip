@@ -16,7 +16,11 @@ using namespace rofn;
 constexpr int kMaxNormColumns = ROF_LAYER_NORM_MAX_COLUMNS;
 // Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.
 constexpr int kBackwardBlocks = 1024;
-constexpr int kForwardBlocks = 2048;
+// An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
+constexpr int64_t kStreamOutBytes = 128 << 20;
+constexpr int kDropoutBlocks = 2048;
+// A launch holds fewer than 2^32 threads.
+constexpr int64_t kMostBlocks = 1 << 22;
 
 struct DropoutArgs {
     const void *x;
@@ -42,25 +46,22 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
         T *dst = (T *)a.out + row * a.ldo + col;
         uint32_t w[4];
         philox_words((uint64_t)i, d, w);
+        Packed<T, 8> data;
         float v[8];
-        if (left >= 8) {
-            load_vec<T, 8>(src, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = e < left ? load_one(src + e) : 0.f;
-        }
+        if (left >= 8)
+            data.load(src);
+        else
+            data.load_few(src, left);
+        data.unpack(v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t u = e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-            v[e] = u >= d.threshold ? v[e] * d.scale : 0.f;
+            if (a.threshold) v[e] = drop_keeps(w[e / 2], e, d) ? v[e] * a.scale : 0.f;
         }
-        if (left >= 8) {
-            store_vec<T, 8>(dst, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < left) store_one(dst + e, v[e]);
-        }
+        data.pack(v);
+        if (left >= 8)
+            data.store(dst);
+        else
+            data.store_part(dst, a.f % 8);
     }
 }
 
@@ -108,24 +109,71 @@ int drop_threshold(const rof_dropout_opts *d) {
 }
 float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.f; }
 
+// The variant for f columns.  A row of up to 64 vectors of 16 bytes is one vector in each lane of the smallest lane group
+// that holds it: few registers, and the rows of a wavefront are one contiguous piece.  Measured (us, forward / backward):
+//   2^20 x 64 bfloat16, 8 vectors: 8 lanes 41 / 66, 4 lanes with two vectors 40 / 79, 16 lanes half empty 53 / 97;
+//   2^18 x 256 float32, 64 vectors: 64 lanes 105 / 165, 32 lanes with two vectors 104 / 173.
+// Above that two or three vectors per lane and as few wavefronts as that takes, because every wavefront more waits for the
+// others twice per row (2048 bfloat16 columns, 256 vectors, 80 M elements: one wavefront with four vectors 57 / 95, two with
+// two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90).
 NormShape norm_shape(int f, int x_dtype) {
+    static const struct { int most, lpr, waves, k; } kShapes[] = {
+        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},     {16, 16, 1, 1},   {32, 32, 1, 1},   {64, 64, 1, 1},  {128, 64, 1, 2},
+        {192, 64, 1, 3}, {256, 64, 2, 2}, {512, 64, 4, 2}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}, {3072, 64, 16, 3}, {4096, 64, 16, 4}};
     const int vecs = (f * size_of(x_dtype) + 15) / 16;
-    NormShape s;
-    s.lpr = 64;
-    s.waves = vecs <= 256 ? 1 : vecs <= 1024 ? 4 : 16;
-    s.k = (vecs + s.lpr * s.waves - 1) / (s.lpr * s.waves);
-    s.rows = (s.waves > 4 ? s.waves * 64 : 256) / (s.lpr * s.waves);
+    NormShape s = {0, 0, 0, false};
+    for (const auto &c : kShapes)
+        if (!s.k && vecs <= c.most) s = {c.lpr, c.waves, c.k, false};
     return s;
 }
 
-int blocks_for(int64_t n, const NormShape &s, int most) {
-    return (int)std::min<int64_t>((n + s.rows - 1) / s.rows, s.waves > 4 ? most / 4 : most);
+// How many workgroups, and which rows each takes.
+// Forward: workgroups of four consecutive rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
+// with 2048 workgroups that stay and step through the matrix together; at 2.4 M x 47 float32 195 / 206), else as many as stay.
+// Backward: each workgroup leaves a row of partial sums, so they are those that stay: 1024 of up to 256 threads, half as many
+// where the lanes hold several vectors (their registers leave room for no more).
+int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
+    const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
+    const bool lean = s.waves == 2 || (s.waves == 1 && s.k == 1);
+    if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
+        a.chunk = a.span = 4 * rows;
+        a.step = rows;
+        return (int)((rounds + 3) / 4);
+    }
+    const int blocks = (int)std::min<int64_t>(rounds, backward ? (lean ? kBackwardBlocks : kBackwardBlocks / 2) : (lean ? 2048 : 1024));
+    a.chunk = rows;
+    a.step = blocks * rows;
+    a.span = a.n;
+    return blocks;
 }
 
-int launch_norm(const NormArgs &a, int x_dtype, int y_dtype, bool backward, const NormShape &s, int blocks, hipStream_t st) {
-    if (x_dtype == ROF_F32)
-        return y_dtype == ROF_F32 ? launch_norm_f32_f32(a, backward, s, blocks, st) : launch_norm_f32_bf16(a, backward, s, blocks, st);
-    return y_dtype == ROF_F32 ? launch_norm_bf16_f32(a, backward, s, blocks, st) : launch_norm_bf16_bf16(a, backward, s, blocks, st);
+// Streaming accesses in the backward launch: where its result is larger than the caches keep until its consumer runs, its
+// inputs are read for the last time as well, and whole rows are whole cache lines (2^18 x 256 float32: 165 us against 176,
+// 2^20 x 64 bfloat16 66 / 74; rows of 47 columns, whose lines two wavefronts share, 322 / 305).
+bool norm_streams(const NormArgs &a, const NormShape &s, int x_dtype, int y_dtype) {
+    const int sx = size_of(x_dtype), sy = size_of(y_dtype);
+    if (a.n * a.f * sx < kStreamOutBytes || s.k > 2 || s.lpr < 8) return false;
+    return aligned(a.x, 16) && aligned(a.dout, 16) && aligned(a.out, 16) && a.ldx * sx % 16 == 0 && a.ldd * sy % 16 == 0 &&
+           a.ldo * sx % 16 == 0 && (int64_t)a.f * sx % 16 == 0;
+}
+
+int launch_norm(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st) {
+    const NormShape s = norm_shape(a.f, x_dtype);
+    const int blocks = norm_blocks(a, s, false);
+    if (x_dtype == ROF_F32) return y_dtype == ROF_F32 ? norm_fwd_f32_f32(a, s, blocks, st) : norm_fwd_f32_bf16(a, s, blocks, st);
+    return y_dtype == ROF_F32 ? norm_fwd_bf16_f32(a, s, blocks, st) : norm_fwd_bf16_bf16(a, s, blocks, st);
+}
+
+int launch_norm_backward(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st, int *blocks) {
+    NormShape s = norm_shape(a.f, x_dtype);
+    s.stream = norm_streams(a, s, x_dtype, y_dtype);
+    const int b = *blocks = norm_blocks(a, s, true);
+    if (x_dtype == ROF_F32) {
+        if (y_dtype == ROF_F32) return a.relu ? norm_bwd_relu_f32_f32(a, s, b, st) : norm_bwd_f32_f32(a, s, b, st);
+        return a.relu ? norm_bwd_relu_f32_bf16(a, s, b, st) : norm_bwd_f32_bf16(a, s, b, st);
+    }
+    if (y_dtype == ROF_F32) return a.relu ? norm_bwd_relu_bf16_f32(a, s, b, st) : norm_bwd_bf16_f32(a, s, b, st);
+    return a.relu ? norm_bwd_relu_bf16_bf16(a, s, b, st) : norm_bwd_bf16_bf16(a, s, b, st);
 }
 
 // the arguments that the two directions share
@@ -186,7 +234,7 @@ int rof_dropout(const void *x, int dtype, int64_t ldx, int64_t n, int f, void *o
     a.scale = drop_scale(t);
     a.state = t > 0 ? dropout->state : nullptr;
     a.call = dropout->call;
-    const int blocks = (int)std::min<int64_t>((a.items + 255) / 256, kForwardBlocks);
+    const int blocks = (int)std::min<int64_t>((a.items + 255) / 256, kDropoutBlocks);
     if (dtype == ROF_F32)
         hipLaunchKernelGGL(dropout_kernel<float>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
     else
@@ -204,8 +252,7 @@ int rof_layer_norm(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, co
     if (n == 0) return ROF_OK;
     a.out = out;
     a.ldo = ldo;
-    const NormShape s = norm_shape(f, x_dtype);
-    return launch_norm(a, x_dtype, out_dtype, false, s, blocks_for(n, s, kForwardBlocks), (hipStream_t)stream);
+    return launch_norm(a, x_dtype, out_dtype, (hipStream_t)stream);
 }
 
 size_t rof_layer_norm_backward_workspace_bytes(int64_t n, int f) {
@@ -227,15 +274,14 @@ int rof_layer_norm_backward(const void *dout, int dout_dtype, int64_t ldd, const
     if (params && n && (!workspace || !aligned(workspace, 16) || workspace_bytes < rof_layer_norm_backward_workspace_bytes(n, f)))
         return ROF_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
-    const NormShape s = norm_shape(f, x_dtype);
-    const int blocks = blocks_for(n, s, kBackwardBlocks);
+    int blocks = 0;
     if (n && (params || dx)) {
         a.dout = dout;
         a.ldd = ldd;
         a.out = dx;
         a.ldo = lddx;
         a.partial = params ? (float *)workspace : nullptr;
-        const int status = launch_norm(a, x_dtype, dout_dtype, true, s, blocks, st);
+        const int status = launch_norm_backward(a, x_dtype, dout_dtype, st, &blocks);
         if (status) return status;
     }
     if (params) {
