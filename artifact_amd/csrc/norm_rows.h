@@ -283,19 +283,32 @@ struct RowMap {
     }
 };
 
-// Where a lane's row begins, from one round of the launch to the next; it stays on its last row when the next would be
-// behind the matrix.  `all` (the same in every lane): no lane of the workgroup is that far, which spares the choice.
+// The rounds of a workgroup: `inner` of them next to each other, then the same again a whole launch further on.
+struct Rounds {
+    int64_t left;      // rows from this round's first one to the matrix's end
+    int64_t step;      // rows from this round to the next
+    int32_t in;
+    template <int ROWS>
+    __device__ __forceinline__ static int64_t first(const NormArgs &a) { return (int64_t)blockIdx.x * a.inner * ROWS; }
+    __device__ __forceinline__ Rounds(const NormArgs &a, int64_t first, int rows) : left(a.n - first), in(a.inner) { plan(a, rows); }
+    __device__ __forceinline__ void plan(const NormArgs &a, int rows) { step = in == 1 ? a.jump : rows; }
+    __device__ __forceinline__ void next(const NormArgs &a, int rows) {
+        left -= step;
+        in = in == 1 ? a.inner : in - 1;
+        plan(a, rows);
+    }
+};
+
+// Where a lane's row begins, from one round to the next; it stays on its last row when the next would be behind the matrix.
+// `all` (the same in every lane): no lane of the workgroup is that far, which spares the choice.
 template <typename T>
 struct Cursor {
     T *at;
-    int64_t stride;
-    __device__ __forceinline__ Cursor(T *base, int64_t ld, int64_t row, int64_t rows, int64_t step)
-        : at(base + (row < rows ? row : rows - 1) * ld), stride(step * ld) {}
-    __device__ __forceinline__ void advance(bool all, bool further) {
-        if (all)
-            at += stride;
-        else if (further)
-            at += stride;
+    int64_t ld;
+    __device__ __forceinline__ Cursor(T *base, int64_t ld_, int64_t row, int64_t rows)
+        : at(base + (row < rows ? row : rows - 1) * ld_), ld(ld_) {}
+    __device__ __forceinline__ void advance(int64_t step, bool all, bool further) {
+        if (all || further) at += step * ld;
     }
 };
 
@@ -371,19 +384,20 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
     const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, most, a.scale), bias(m, a.bias, 0.f, 0.f, bstore, most, a.scale);
     const Drop drop(a);
     const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
-    const int64_t step = a.step, first = (int64_t)blockIdx.x * a.chunk, stop = std::min(a.n, first + a.span);
+    const int64_t first = Rounds::first<Map::ROWS>(a);
+    Rounds go(a, first, Map::ROWS);
     const uint32_t groups = (uint32_t)(a.f + 7) / 8;
     typename Map::template Part<TX> next;
     const int64_t row = first + m.slot;
     uint64_t group = (uint64_t)row * groups;
-    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n, step);
-    Cursor<TY> out((TY *)a.out, a.ldo, row, a.n, step);
+    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n);
+    Cursor<TY> out((TY *)a.out, a.ldo, row, a.n);
     next.template load<false>(m, x.at);
-    for (int64_t left = stop - first; left > 0; left -= step) {
-        const bool ok = m.slot < left, all = step + Map::ROWS <= left, further = m.slot + step < left;
+    for (; go.left > 0; go.next(a, Map::ROWS)) {
+        const bool ok = m.slot < go.left, all = go.step + Map::ROWS <= go.left, further = m.slot + go.step < go.left;
         float v[K][V];
         next.unpack(m, v);
-        x.advance(all, further);
+        x.advance(go.step, all, further);
         next.template load<false>(m, x.at);   // on its way while this row is worked on
         float mean, squares;
         m.moments(v, f, inv_f, sh.part, turn, mean, squares);
@@ -407,8 +421,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
         }
         next.arrive();
         if (ok) m.template store<false>(out.at, v);
-        out.advance(all, further);
-        group += (uint64_t)step * groups;
+        out.advance(go.step, all, further);
+        group += (uint64_t)go.step * groups;
     }
 }
 
@@ -504,29 +518,30 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
         for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.f;
     const Drop drop(a);
     const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
-    const int64_t step = a.step, first = (int64_t)blockIdx.x * a.chunk, stop = std::min(a.n, first + a.span);
+    const int64_t first = Rounds::first<Map::ROWS>(a);
+    Rounds go(a, first, Map::ROWS);
     const uint32_t groups = (uint32_t)(a.f + 7) / 8;
     typename Map::template Part<TX> next_x;
     typename Map::template Part<TY> next_d;
     const int64_t row = first + m.slot;
     uint64_t group = (uint64_t)row * groups;
-    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n, step);
-    Cursor<const TY> dout((const TY *)a.dout, a.ldd, row, a.n, step);
-    Cursor<TX> dx((TX *)a.out, a.ldo, row, a.n, step);
+    Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n);
+    Cursor<const TY> dout((const TY *)a.dout, a.ldd, row, a.n);
+    Cursor<TX> dx((TX *)a.out, a.ldo, row, a.n);
     next_x.template load<STREAM>(m, x.at);
     next_d.template load<STREAM>(m, dout.at);
-    for (int64_t left = stop - first; left > 0; left -= step) {
-        const bool ok = m.slot < left, all = step + Map::ROWS <= left, further = m.slot + step < left;
+    for (; go.left > 0; go.next(a, Map::ROWS)) {
+        const bool ok = m.slot < go.left, all = go.step + Map::ROWS <= go.left, further = m.slot + go.step < go.left;
         float h[K][V], d[K][V];
         next_x.unpack(m, h);
         next_d.unpack(m, d);
         const TX *const here = x.at;
-        x.advance(all, further);   // on their way while this row is worked on
-        dout.advance(all, further);
+        x.advance(go.step, all, further);   // on their way while this row is worked on
+        dout.advance(go.step, all, further);
         next_x.template load<STREAM>(m, x.at);
         next_d.template load<STREAM>(m, dout.at);
         // (columns that do not exist hold other columns of d: their weight is 0, and their sums are not stored)
-        if (left < Map::ROWS) {   // lane groups behind the last row work on it once more and add nothing
+        if (go.left < Map::ROWS) {   // lane groups behind the last row work on it once more and add nothing
 #pragma unroll
             for (int j = 0; j < K; ++j)
 #pragma unroll
@@ -595,9 +610,9 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 #pragma unroll
                 for (int e = 0; e < V; ++e) d[j][e] = fmaf(h[j][e], s2, fmaf(d[j][e], rs, s1));
             if (ok) m.template store<STREAM>(dx.at, d);
-            dx.advance(all, further);
+            dx.advance(go.step, all, further);
         }
-        group += (uint64_t)step * groups;
+        group += (uint64_t)go.step * groups;
     }
     if (!a.partial) return;
 #pragma unroll

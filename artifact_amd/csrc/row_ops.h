@@ -19,7 +19,8 @@ struct NormArgs {
     float *partial;          // backward: [workgroups][2][f], or null
     int64_t ldx, ldd, ldo;
     int64_t n;
-    int64_t chunk, step, span;   // workgroup i works on the rows i chunk ... + span, `step` of them apart from one round to the next
+    int64_t jump;            // rows from the last of a workgroup's adjacent rounds to its next round
+    int32_t inner;           // adjacent rounds
     int32_t f;
     int32_t relu;
     int32_t drop;            // dropout on

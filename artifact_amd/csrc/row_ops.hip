@@ -14,11 +14,14 @@ namespace {
 using namespace rofn;
 
 constexpr int kMaxNormColumns = ROF_LAYER_NORM_MAX_COLUMNS;
-// Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.
-constexpr int kBackwardBlocks = 1024;
+// Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.  Where there
+// are more rounds of work than kManyRounds it is tiles of eight rounds, see norm_blocks, else workgroups that stay.
+constexpr int kBackwardBlocks = 1024, kBackwardTiles = 16384;
+constexpr int64_t kManyRounds = 65536;
+constexpr int kTiledColumns = 512;   // rows of more columns are several vectors per lane in either type
+constexpr int kParamsChunks = 128;   // rows that the first of two passes leaves of so many partial ones
 // An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
 constexpr int64_t kStreamOutBytes = 128 << 20;
-constexpr int kDropoutBlocks = 2048;
 // A launch holds fewer than 2^32 threads.
 constexpr int64_t kMostBlocks = 1 << 22;
 
@@ -26,42 +29,76 @@ struct DropoutArgs {
     const void *x;
     void *out;
     int64_t ldx, ldo;
-    int64_t items;           // rows times groups of eight columns
-    int32_t f, groups;
+    int64_t n;
+    int64_t tiles;
+    int32_t f;
+    int32_t vecs;            // vectors of 16 bytes per row
+    int32_t rows, parts;     // a tile is `rows` whole rows (parts = 1) or one of the `parts` parts of a row
+    uint32_t magic;          // floor(2^32 / vecs) + 1 (0: a row is one vector)
     uint32_t threshold;
     float scale;
     const int64_t *state;
     int64_t call;
 };
 
-// One thread per group of eight columns, that is per call of the generator.
-template <typename T>
+// A workgroup's tile is 1024 vectors (four per lane, loaded together) of whole rows next to each other, or a part of one long
+// row.  Bounded by memory: half of its operations are the generator's (a call per vector; two float32 vectors make the same
+// call, which is cheaper than eight columns per lane, whose loads would be 32 bytes apart).  Tiles rather than workgroups that
+// stay and step through the matrix: 2^22 x 256 bfloat16 695 us a pass against 900, 2.4 M x 100 float32 347 against 450.
+constexpr int kTileVecs = 1024;
+
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), U = kTileVecs / 256;
     const Drop d(a);
-    const int64_t step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.items; i += step) {
-        const int64_t row = i / a.groups;
-        const int col = (int)(i - row * a.groups) * 8, left = a.f - col;
-        const T *src = (const T *)a.x + row * a.ldx + col;
-        T *dst = (T *)a.out + row * a.ldo + col;
-        uint32_t w[4];
-        philox_words((uint64_t)i, d, w);
-        Packed<T, 8> data;
-        float v[8];
-        if (left >= 8)
-            data.load(src);
-        else
-            data.load_few(src, left);
-        data.unpack(v);
+    const uint32_t groups = (uint32_t)(a.f + 7) / 8;
+    const int tail = a.f % V;
+    for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+        const int64_t row0 = a.parts > 1 ? tile / a.parts : tile * a.rows;
+        const uint32_t vec0 = a.parts > 1 ? (uint32_t)(tile - row0 * a.parts) * kTileVecs : 0;
+        const uint32_t count = a.parts > 1 ? std::min((uint32_t)a.vecs - vec0, (uint32_t)kTileVecs)
+                                           : (uint32_t)std::min<int64_t>(a.n - row0, a.rows) * (uint32_t)a.vecs;
+        const T *const src = (const T *)a.x + row0 * a.ldx;
+        T *const dst = (T *)a.out + row0 * a.ldo;
+        const uint64_t group0 = (uint64_t)row0 * groups;
+        Packed<T, V> p[U];
+        uint32_t row[U], col[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (a.threshold) v[e] = drop_keeps(w[e / 2], e, d) ? v[e] * a.scale : 0.f;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = std::min(u * 256 + threadIdx.x, count - 1);   // behind the tile: its last vector once more, not stored
+            row[u] = a.parts > 1 ? 0 : a.magic ? __umulhi(i, a.magic) : i;   // i / vecs: exact, since i and vecs are at most 1024
+            col[u] = (vec0 + i - row[u] * (uint32_t)a.vecs) * V;
+            const T *const at = src + (uint64_t)row[u] * (uint64_t)a.ldx;
+            // the last vector of a row that is no multiple of V: read from the row's end and shifted into place
+            if (a.f < V)
+                p[u].load_few(at, a.f);
+            else
+                p[u].template load<STREAM>(at + std::min(col[u], (uint32_t)(a.f - V)));
         }
-        data.pack(v);
-        if (left >= 8)
-            data.store(dst);
-        else
-            data.store_part(dst, a.f % 8);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool cut = col[u] + V > (uint32_t)a.f;
+            if (tail && a.f >= V) p[u].shift(cut ? V - tail : 0);
+            float v[V];
+            p[u].unpack(v);
+            if (a.threshold) {
+                uint32_t w[4];
+                philox_words(group0 + (uint64_t)row[u] * groups + col[u] / 8, d, w);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const uint32_t word = V == 4 && (col[u] & 4) ? w[(2 + e / 2) % 4] : w[e / 2];
+                    v[e] = drop_keeps(word, e, d) ? v[e] * a.scale : 0.f;
+                }
+            }
+            p[u].pack(v);
+            if (u * 256 + threadIdx.x < count) {
+                T *const at = dst + (uint64_t)row[u] * (uint64_t)a.ldo + col[u];
+                if (cut)
+                    p[u].store_part(at, tail);
+                else
+                    p[u].template store<STREAM>(at);
+            }
+        }
     }
 }
 
@@ -96,6 +133,23 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restri
     }
 }
 
+// Thousands of partial rows are first added up in kParamsChunks chunks, 64 columns of a chunk per workgroup.
+__global__ __launch_bounds__(256) void norm_params_chunk_kernel(const float *__restrict__ partial, int blocks, int f,
+                                                                 float *__restrict__ out) {
+    __shared__ float red[4][64];
+    const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+    const int c = blockIdx.x * 64 + tx, per = (blocks + kParamsChunks - 1) / kParamsChunks;
+    const int first = blockIdx.y * per, last = std::min(blocks, first + per);
+    float s = 0.f;
+    if (c < 2 * f) {
+#pragma unroll 8
+        for (int b = first + ty; b < last; b += 4) s += partial[(int64_t)b * 2 * f + c];
+    }
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < 2 * f) out[(int64_t)blockIdx.y * 2 * f + c] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+}
+
 bool known_type(int t) { return t == ROF_F32 || t == ROF_BF16; }
 int size_of(int t) { return t == ROF_F32 ? 4 : 2; }
 bool aligned(const void *p, int size) { return ((uintptr_t)p) % (uintptr_t)size == 0; }
@@ -127,23 +181,30 @@ NormShape norm_shape(int f, int x_dtype) {
     return s;
 }
 
-// How many workgroups, and which rows each takes.
-// Forward: workgroups of four consecutive rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
-// with 2048 workgroups that stay and step through the matrix together; at 2.4 M x 47 float32 195 / 206), else as many as stay.
-// Backward: each workgroup leaves a row of partial sums, so they are those that stay: 1024 of up to 256 threads, half as many
-// where the lanes hold several vectors (their registers leave room for no more).
+// How many workgroups, and which rounds each takes.
+// Forward: a workgroup per four adjacent rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
+// with 2048 workgroups that stay and step through the matrix together; 2.4 M x 47 float32 192 / 206), else as many as stay.
+// Backward: each workgroup leaves a row of partial sums.  With many rounds it is up to 16384 tiles of eight adjacent ones,
+// handed out as others end (2^22 x 256 bfloat16: 1221 us against 1355 with 1024 workgroups that stay, 2.4 M x 47 float32
+// 268 / 305, 10^6 x 100 243 / 275); with fewer 1024 that stay (2^20 x 64 bfloat16: 66 / 73), half as many where the lanes
+// hold several vectors, whose registers leave room for no more, and two adjacent rounds at a time (20011 x 4099 bfloat16:
+// 106 us against 117 one at a time; forward 73 / 80).
 int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
     const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
-    const bool lean = s.waves == 2 || (s.waves == 1 && s.k == 1);
+    const bool lean = s.waves == 1 && s.k == 1;
+    int64_t most;
     if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
-        a.chunk = a.span = 4 * rows;
-        a.step = rows;
-        return (int)((rounds + 3) / 4);
+        a.inner = 4;
+        most = kMostBlocks;
+    } else if (backward && lean && rounds >= kManyRounds) {
+        a.inner = 8;
+        most = kBackwardTiles;
+    } else {
+        a.inner = lean || rounds < 2048 ? 1 : 2;
+        most = backward ? (lean || s.waves == 2 ? kBackwardBlocks : kBackwardBlocks / 2) : 2048;
     }
-    const int blocks = (int)std::min<int64_t>(rounds, backward ? (lean ? kBackwardBlocks : kBackwardBlocks / 2) : (lean ? 2048 : 1024));
-    a.chunk = rows;
-    a.step = blocks * rows;
-    a.span = a.n;
+    const int blocks = (int)std::min<int64_t>((rounds + a.inner - 1) / a.inner, most);
+    a.jump = ((int64_t)blocks * a.inner - (a.inner - 1)) * rows;
     return blocks;
 }
 
@@ -216,7 +277,7 @@ int rof_dropout_state_next(int64_t *state, int64_t calls, int64_t *used, void *s
 }
 
 int rof_dropout(const void *x, int dtype, int64_t ldx, int64_t n, int f, void *out, int64_t ldo,
-                const rof_dropout_opts *dropout, void *stream) {
+                const rof_dropout_opts *dropout, void *stream_) {
     if (!dropout || n < 0 || f < 1 || ldx < f || ldo < f || (n && (!x || !out))) return ROF_ERR_ARG;
     if (!known_type(dtype)) return ROF_ERR_UNSUPPORTED;
     const int t = drop_threshold(dropout);
@@ -227,18 +288,30 @@ int rof_dropout(const void *x, int dtype, int64_t ldx, int64_t n, int f, void *o
     a.out = out;
     a.ldx = ldx;
     a.ldo = ldo;
+    a.n = n;
     a.f = f;
-    a.groups = (f + 7) / 8;
-    a.items = n * a.groups;
+    const int per = 16 / size_of(dtype);
+    a.vecs = f / per + (f % per != 0);
+    a.rows = std::max(1, kTileVecs / a.vecs);
+    a.parts = (a.vecs + kTileVecs - 1) / kTileVecs;
+    a.tiles = a.parts > 1 ? n * a.parts : (n + a.rows - 1) / a.rows;
+    a.magic = a.vecs > 1 ? (uint32_t)(((uint64_t)1 << 32) / a.vecs) + 1 : 0;
     a.threshold = (uint32_t)t;
     a.scale = drop_scale(t);
     a.state = t > 0 ? dropout->state : nullptr;
     a.call = dropout->call;
-    const int blocks = (int)std::min<int64_t>((a.items + 255) / 256, kDropoutBlocks);
-    if (dtype == ROF_F32)
-        hipLaunchKernelGGL(dropout_kernel<float>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+    const bool stream = n * f * size_of(dtype) >= kStreamOutBytes && aligned(x, 16) && aligned(out, 16) && f % per == 0 &&
+                        ldx % per == 0 && ldo % per == 0;
+    const dim3 grid((unsigned)std::min(a.tiles, kMostBlocks));
+    hipStream_t st = (hipStream_t)stream_;
+    if (dtype == ROF_F32 && stream)
+        hipLaunchKernelGGL((dropout_kernel<float, true>), grid, dim3(256), 0, st, a);
+    else if (dtype == ROF_F32)
+        hipLaunchKernelGGL((dropout_kernel<float, false>), grid, dim3(256), 0, st, a);
+    else if (stream)
+        hipLaunchKernelGGL((dropout_kernel<bf16_t, true>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL(dropout_kernel<bf16_t>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL((dropout_kernel<bf16_t, false>), grid, dim3(256), 0, st, a);
     HIP_TRY(hipGetLastError());
     return ROF_OK;
 }
@@ -257,7 +330,8 @@ int rof_layer_norm(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, co
 
 size_t rof_layer_norm_backward_workspace_bytes(int64_t n, int f) {
     if (n <= 0 || f <= 0) return 0;
-    return (size_t)std::min<int64_t>(n, kBackwardBlocks) * 2 * (size_t)f * sizeof(float);
+    const int64_t rows = n >= kManyRounds && f <= kTiledColumns ? kBackwardTiles + kParamsChunks : std::min<int64_t>(n, kBackwardBlocks);
+    return (size_t)rows * 2 * (size_t)f * sizeof(float);
 }
 
 int rof_layer_norm_backward(const void *dout, int dout_dtype, int64_t ldd, const void *x, int x_dtype, int64_t ldx, int64_t n,
@@ -285,8 +359,16 @@ int rof_layer_norm_backward(const void *dout, int dout_dtype, int64_t ldd, const
         if (status) return status;
     }
     if (params) {
-        hipLaunchKernelGGL(norm_params_kernel, dim3((2 * f + 15) / 16), dim3(1024), 0, st, (const float *)workspace, blocks, f,
-                           dweight, dbias);
+        const float *partial = (const float *)workspace;
+        if (blocks > kBackwardBlocks) {
+            float *chunks = (float *)workspace + (int64_t)kBackwardTiles * 2 * f;
+            hipLaunchKernelGGL(norm_params_chunk_kernel, dim3((2 * f + 63) / 64, kParamsChunks), dim3(256), 0, st, partial, blocks, f,
+                               chunks);
+            HIP_TRY(hipGetLastError());
+            partial = chunks;
+            blocks = kParamsChunks;
+        }
+        hipLaunchKernelGGL(norm_params_kernel, dim3((2 * f + 15) / 16), dim3(1024), 0, st, partial, blocks, f, dweight, dbias);
         HIP_TRY(hipGetLastError());
     }
     return ROF_OK;

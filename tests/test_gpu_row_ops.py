@@ -9,7 +9,7 @@ import torch
 from artifact_amd import _lib, row_ops
 from artifact_amd._lib import DropoutOpts, RofError
 from artifact_amd.row_ops import ROF_Dropout, ROF_DropoutState, ROF_LayerNorm, dropout, layer_norm
-from row_oracle import HALF_STEP, Norm, kept, scale
+from row_oracle import HALF_STEP, U, Norm, kept, scale
 
 pytestmark = pytest.mark.gpu
 
@@ -98,6 +98,26 @@ def test_the_tail_of_a_hidden_layer_and_its_gradient(n, f, xt, yt, relu, p):
 def test_more_rows_than_one_launch_holds_at_a_time(n, f, dtype):
     w, b = params(f, 3)
     check_norm(rows_of(n, f, dtype, 5), w, b, rows_of(n, f, dtype, 6), True, 0.5)
+
+
+@pytest.mark.parametrize("dtype,n,f", [("float32", (1 << 18) + 3, 200), ("bfloat16", (1 << 18) + 77, 500), ("float32", (1 << 20) + 5, 33)])
+def test_parameter_gradients_of_matrices_in_tiles(dtype, n, f):
+    """So many rows that the backward launch leaves thousands of partial rows, which two more launches add up.  The 64-bit
+    form is evaluated on the GPU here; the tolerances are row_oracle's."""
+    x, dy = rows_of(n, f, dtype, 1, mean=0.0).requires_grad_(True), rows_of(n, f, dtype, 2)
+    w, b = params(f, 3)
+    dx, dw, db = torch.autograd.grad(layer_norm(x, w, b), (x, w, b), dy)
+    x64, d = x.detach().double(), dy.double()
+    m = x64.mean(1, keepdim=True)
+    r = 1 / torch.sqrt(((x64 - m) ** 2).mean(1, keepdim=True) + 1e-5)
+    h, a = (x64 - m) * r, 128 * U * (r * (x64.abs() + m.abs()) + 1)
+    adds = -(-n // 1024) + 104
+    near(dw, host((d * h).sum(0)), host((d.abs() * a).sum(0) + adds * U * (d * h).abs().sum(0)), "dweight")
+    near(db, host(d.sum(0)), host(adds * U * d.abs().sum(0)), "dbias")
+    rows = [0, 1, n // 2, n - 2, n - 1]
+    o = Norm(host(x[rows]), host(w), host(b))
+    want, tol = o.backward(host(dy[rows]))
+    near(dx[rows], want[0], tol[0], "dx")
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
