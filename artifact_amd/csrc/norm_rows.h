@@ -272,15 +272,6 @@ struct RowMap {
             for (int e = 0; e < V; ++e) v[K - 1][e] = has(K - 1, e) ? v[K - 1][e] : 0.f;
         }
     }
-
-    // The elements of a vector that the dropout keeps; `group` is the row's first.  A vector is a whole group of eight columns
-    // or half of one.
-    __device__ __forceinline__ void kept(const Drop &d, uint64_t group, int j, bool (&keep)[V]) const {
-        uint32_t w[4];
-        philox_words(group + (uint32_t)(col(j) / 8), d, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) keep[e] = drop_keeps(V == 4 && (col(j) & 4) ? w[(2 + e / 2) % 4] : w[e / 2], e, d);
-    }
 };
 
 // The rounds of a workgroup: `inner` of them next to each other, then the same again a whole launch further on.
@@ -414,7 +405,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
             }
             if (a.drop) {
                 bool keep[V];
-                m.kept(drop, group, j, keep);
+                drop_kept(drop, group, (uint32_t)m.col(j), keep);
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[j][e] = keep[e] ? v[j][e] : 0.f;
             }
@@ -558,7 +549,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 #pragma unroll
             for (int j = 0; j < K; ++j) {
                 bool keep[V];
-                m.kept(drop, group, j, keep);
+                drop_kept(drop, group, (uint32_t)m.col(j), keep);
 #pragma unroll
                 for (int e = 0; e < V; ++e) d[j][e] = keep[e] ? d[j][e] : 0.f;
             }

@@ -92,6 +92,23 @@ __device__ __forceinline__ void philox_words(uint64_t group, const Drop &d, uint
     w[3] = c3;
 }
 
+// The elements of a vector of V columns from `col` on that the dropout keeps; `group` is the row's first.  A vector is a whole
+// group of eight columns or half of one: the half's words are chosen as values (an index into the array would put it into
+// memory, and a kernel that has to place memory per lane starts by asking the host for its launch shape: 14 us).
+template <int V>
+__device__ __forceinline__ void drop_kept(const Drop &d, uint64_t group, uint32_t col, bool (&keep)[V]) {
+    uint32_t w[4];
+    philox_words(group + col / 8, d, w);
+    if constexpr (V == 4) {
+        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+        const bool upper = col & 4;
+        w[0] = upper ? w2 : w0;
+        w[1] = upper ? w3 : w1;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) keep[e] = drop_keeps(w[e / 2], e, d);
+}
+
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 

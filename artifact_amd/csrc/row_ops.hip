@@ -44,7 +44,7 @@ struct DropoutArgs {
 // A workgroup's tile is 1024 vectors (four per lane, loaded together) of whole rows next to each other, or a part of one long
 // row.  Bounded by memory: half of its operations are the generator's (a call per vector; two float32 vectors make the same
 // call, which is cheaper than eight columns per lane, whose loads would be 32 bytes apart).  Tiles rather than workgroups that
-// stay and step through the matrix: 2^22 x 256 bfloat16 695 us a pass against 900, 2.4 M x 100 float32 347 against 450.
+// stay and step through the matrix: 2^22 x 256 bfloat16 695 us a pass against 900, 2.4 M x 100 float32 318 against 450.
 constexpr int kTileVecs = 1024;
 
 template <typename T, bool STREAM>
@@ -82,13 +82,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
             float v[V];
             p[u].unpack(v);
             if (a.threshold) {
-                uint32_t w[4];
-                philox_words(group0 + (uint64_t)row[u] * groups + col[u] / 8, d, w);
+                bool keep[V];
+                drop_kept(d, group0 + (uint64_t)row[u] * groups, col[u], keep);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const uint32_t word = V == 4 && (col[u] & 4) ? w[(2 + e / 2) % 4] : w[e / 2];
-                    v[e] = drop_keeps(word, e, d) ? v[e] * a.scale : 0.f;
-                }
+                for (int e = 0; e < V; ++e) v[e] = keep[e] ? v[e] * a.scale : 0.f;
             }
             p[u].pack(v);
             if (u * 256 + threadIdx.x < count) {
@@ -183,10 +180,10 @@ NormShape norm_shape(int f, int x_dtype) {
 
 // How many workgroups, and which rounds each takes.
 // Forward: a workgroup per four adjacent rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
-// with 2048 workgroups that stay and step through the matrix together; 2.4 M x 47 float32 192 / 206), else as many as stay.
+// with 2048 workgroups that stay and step through the matrix together; 10^6 x 100 float32 142 / 155), else as many as stay.
 // Backward: each workgroup leaves a row of partial sums.  With many rounds it is up to 16384 tiles of eight adjacent ones,
 // handed out as others end (2^22 x 256 bfloat16: 1221 us against 1355 with 1024 workgroups that stay, 2.4 M x 47 float32
-// 268 / 305, 10^6 x 100 243 / 275); with fewer 1024 that stay (2^20 x 64 bfloat16: 66 / 73), half as many where the lanes
+// 258 / 285, 10^6 x 100 233 / 272); with fewer 1024 that stay (2^20 x 64 bfloat16: 66 / 73), half as many where the lanes
 // hold several vectors, whose registers leave room for no more, and two adjacent rounds at a time (20011 x 4099 bfloat16:
 // 106 us against 117 one at a time; forward 73 / 80).
 int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
@@ -209,8 +206,8 @@ int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
 }
 
 // Streaming accesses in the backward launch: where its result is larger than the caches keep until its consumer runs, its
-// inputs are read for the last time as well, and whole rows are whole cache lines (2^18 x 256 float32: 165 us against 176,
-// 2^20 x 64 bfloat16 66 / 74; rows of 47 columns, whose lines two wavefronts share, 322 / 305).
+// inputs are read for the last time as well, and whole rows are whole cache lines (2^18 x 256 float32: 146 us against 154,
+// 2^20 x 64 bfloat16 66 / 74; rows of 47 columns, whose lines two wavefronts share, 288 / 258).
 bool norm_streams(const NormArgs &a, const NormShape &s, int x_dtype, int y_dtype) {
     const int sx = size_of(x_dtype), sy = size_of(y_dtype);
     if (a.n * a.f * sx < kStreamOutBytes || s.k > 2 || s.lpr < 8) return false;
