@@ -4,8 +4,8 @@
 
 hipcc cross-compiles for gfx950 without a GPU.  The library is loaded with ctypes
 (artifact_amd/_lib.py) and does not link against PyTorch.  `build_torch_module` then compiles the thin
-C++ module `artifact_amd/_ROF*.so` (csrc/rof_torch.cpp: upstream's seven `ROF` operators over the C ABI),
-which links against PyTorch and librof.so.
+C++ modules `artifact_amd/_ROF*.so` (csrc/rof_torch.cpp: upstream's seven `ROF` operators over the C ABI) and
+`artifact_amd/_ROFrows*.so` (csrc/row_ops_torch.cpp: the row operators), which link against PyTorch and librof.so.
 """
 from __future__ import annotations
 
@@ -36,26 +36,13 @@ def _run(cmd):
     subprocess.run(cmd, check=True)
 
 
-def build_library(verbose=True):
-    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
-    gxx = shutil.which("g++") or "g++"
-    inc = ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
-    objdir = os.path.join(HERE, "build")
-    os.makedirs(objdir, exist_ok=True)
-    objs = []
-    for s in HOST_SOURCES:
-        o = os.path.join(objdir, s + ".o")
-        _run([gxx] + HOST_FLAGS + inc + ["-c", os.path.join(CSRC, s), "-o", o])
-        objs.append(o)
-    # the kernel translation units are independent: compile them side by side, as many as there are processors (a unit
-    # takes up to a gigabyte)
-    todo, running = list(HIP_SOURCES), []
-    objs += [os.path.join(objdir, s + ".o") for s in HIP_SOURCES]
+def _run_side_by_side(cmds, most):
+    """Run the commands, at most `most` at a time; the first that fails ends the others."""
+    todo, running = list(cmds), []
     try:
         while todo or running:
-            while todo and len(running) < min(os.cpu_count() or 1, 16):
-                src = todo.pop(0)
-                cmd = [hipcc] + HIP_FLAGS + inc + ["-c", os.path.join(CSRC, src), "-o", os.path.join(objdir, src + ".o")]
+            while todo and len(running) < most:
+                cmd = todo.pop(0)
                 print("+", " ".join(cmd), flush=True)
                 running.append((cmd, subprocess.Popen(cmd)))
             for cmd, pr in list(running):
@@ -67,19 +54,37 @@ def build_library(verbose=True):
     finally:
         for _, pr in running:
             pr.kill()
+
+
+def build_library(verbose=True):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    gxx = shutil.which("g++") or "g++"
+    inc = ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
+    objdir = os.path.join(HERE, "build")
+    os.makedirs(objdir, exist_ok=True)
+    objs = []
+    for s in HOST_SOURCES:
+        o = os.path.join(objdir, s + ".o")
+        _run([gxx] + HOST_FLAGS + inc + ["-c", os.path.join(CSRC, s), "-o", o])
+        objs.append(o)
+    # the kernel translation units are independent: compile them side by side, as many as there are processors
+    cmds = [[hipcc] + HIP_FLAGS + inc + ["-c", os.path.join(CSRC, s), "-o", os.path.join(objdir, s + ".o")] for s in HIP_SOURCES]
+    _run_side_by_side(cmds, min(os.cpu_count() or 1, 16))
+    objs += [os.path.join(objdir, s + ".o") for s in HIP_SOURCES]
     _run([hipcc, "-shared", "-fPIC", "-o", LIB] + objs + ["-fopenmp", "-lgomp"])
     return LIB
 
 
-def torch_module_path():
+def torch_module_path(name="_ROF"):
     import sysconfig
 
-    return os.path.join(HERE, "_ROF" + sysconfig.get_config_var("EXT_SUFFIX"))
+    return os.path.join(HERE, name + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def build_torch_module():
-    """csrc/rof_torch.cpp -> artifact_amd/_ROF<ext suffix>.so with g++ against the installed PyTorch's headers and
-    libraries (host code only: the kernels are in librof.so, found at run time next to the module)."""
+    """csrc/rof_torch.cpp -> artifact_amd/_ROF<ext suffix>.so (upstream's operators) and csrc/row_ops_torch.cpp ->
+    artifact_amd/_ROFrows<ext suffix>.so (the row operators) with g++ against the installed PyTorch's headers and
+    libraries (host code only: the kernels are in librof.so, found at run time next to the modules)."""
     import sysconfig
 
     import torch
@@ -88,17 +93,20 @@ def build_torch_module():
     gxx = shutil.which("g++") or "g++"
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    out = torch_module_path()
-    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=_ROF", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I" + os.path.join(ROOT, "include")]
-    cmd += ["-I" + p for p in cpp_extension.include_paths()] + ["-I" + os.path.join(rocm, "include"),
-                                                                 "-I" + sysconfig.get_paths()["include"]]
-    cmd += [os.path.join(CSRC, "rof_torch.cpp"), "-o", out, "-L" + tlib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
-            "-ltorch_hip", "-ltorch_python", "-L" + HERE, "-l:librof.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib]
-    _run(cmd)
-    return out
+    cmds = []
+    for name, source in (("_ROF", "rof_torch.cpp"), ("_ROFrows", "row_ops_torch.cpp")):
+        cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+               f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I" + os.path.join(ROOT, "include")]
+        cmd += ["-I" + p for p in cpp_extension.include_paths()] + ["-I" + os.path.join(rocm, "include"),
+                                                                     "-I" + sysconfig.get_paths()["include"]]
+        cmd += [os.path.join(CSRC, source), "-o", torch_module_path(name), "-L" + tlib, "-lc10", "-lc10_hip", "-ltorch",
+                "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-L" + HERE, "-l:librof.so", "-Wl,-rpath,$ORIGIN",
+                "-Wl,-rpath," + tlib]
+        cmds.append(cmd)
+    _run_side_by_side(cmds, len(cmds))
+    return torch_module_path()
 
 
 if __name__ == "__main__":

@@ -1,0 +1,278 @@
+// The row operators of include/rof.h as differentiable PyTorch functions: the compiled half of artifact_amd/row_ops.py.
+// They are written in C++ because small graphs are a matter of the host: a step of 16384 x 16 floats is 15 us on the device,
+// and as Python functions the operators' forward and backward calls alone took 147 us of the host's time (here 60, most of it
+// the autograd engine's).
+//
+// Nothing but the inputs is kept for the backward pass.  Checks raise the exception type that set_error_type was given.
+//
+// Built by artifact_amd/build.py into artifact_amd/_ROFrows*.so.
+#include <torch/extension.h>
+
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
+#include <cmath>
+#include <memory>
+#include <mutex>
+#include <optional>
+#include <stdexcept>
+#include <string>
+
+#include "rof.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+PyObject *g_error_type = nullptr;
+
+struct Failure : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+
+void require(bool ok, const char *message) {
+    if (!ok) throw Failure(message);
+}
+void require(bool ok, const char *name, const char *message) {
+    if (!ok) throw Failure(std::string(name) + message);
+}
+
+void check(int rc, const char *what) {
+    if (rc == ROF_OK) return;
+    std::string msg = std::string("librof: ") + what + ": " + rof_strerror(rc);
+    if (rc == ROF_ERR_DEVICE) msg += std::string(": ") + rof_last_device_error();
+    throw Failure(msg + " (status " + std::to_string(rc) + ")");
+}
+
+void *current_stream(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+int type_of(at::ScalarType t) { return t == at::kFloat ? ROF_F32 : ROF_BF16; }
+bool known(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
+int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+bool rows_apart(const Tensor &t) {
+    return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+void check_rows(const char *name, const Tensor &t) {
+    require(t.is_cuda() && t.dim() == 2 && known(t.scalar_type()), name, " must be a 2-D float32 or bfloat16 CUDA tensor");
+    require(t.size(1) > 0 && t.size(1) <= INT32_MAX, name, " must have at least one column");
+    require(rows_apart(t), name, " must have unit column stride and rows that do not overlap");
+}
+void check_param(const char *name, const Tensor &t, const Tensor &x) {
+    require(!t.defined() || (t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 1 &&
+                             t.numel() == x.size(1) && t.is_contiguous()),
+            name, " must be a contiguous float32 vector with one element per column on the device of x");
+}
+void check_rate(double p) { require(p >= 0.0 && p <= 1.0, "a dropout rate must lie between 0 and 1"); }
+void check_rng(const Tensor &rng, const Tensor &x) {
+    require(rng.defined(), "dropout needs rng: an int64 tensor {seed, offset} on the device of x (see ROF_DropoutState)");
+    require(rng.scalar_type() == at::kLong && rng.device() == x.device() && rng.numel() == 2 && rng.is_contiguous(),
+            "rng must be a contiguous int64 tensor of two elements {seed, offset} on the device of x");
+}
+
+// An incoming gradient as rows the kernels take: autograd hands over broadcast and transposed ones as well.
+Tensor gradient_rows(Tensor grad, at::ScalarType type) {
+    if (grad.scalar_type() != type) grad = grad.to(type);
+    return rows_apart(grad) ? grad : grad.contiguous();
+}
+
+// Gradients of a pass that is itself recorded (create_graph): differentiating them is an error, not a silent zero.
+variable_list once(variable_list grads, const char *what) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (auto &g : grads)
+        if (g.defined()) {
+            auto fail = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", 1);
+            g = g.detach();
+            g.set_requires_grad(true);
+            g = (*fail)({g})[0];
+        }
+    return grads;
+}
+
+struct DropoutArgs {
+    double p = 0.0;
+    int64_t call = 0;
+};
+
+Tensor run_dropout(const Tensor &x, const DropoutArgs &d, const Tensor &rng) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor out = at::empty({x.size(0), x.size(1)}, x.options());
+    const rof_dropout_opts opts = {d.p, (const int64_t *)rng.data_ptr(), d.call};
+    check(rof_dropout(x.data_ptr(), type_of(x.scalar_type()), row_stride(x), x.size(0), (int)x.size(1), out.data_ptr(), x.size(1),
+                      &opts, current_stream(x)),
+          "dropout");
+    return out;
+}
+
+struct RofDropoutBackward : public Node {
+    SavedVariable rng;
+    DropoutArgs args;
+    at::ScalarType type;
+
+    variable_list apply(variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(1);
+        Tensor dx;
+        {
+            at::NoGradGuard quiet;
+            dx = run_dropout(gradient_rows(grads[0], type), args, rng.unpack());
+        }
+        return once({dx}, "dropout");
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        rng.reset_data();
+    }
+    std::string name() const override { return "RofDropoutBackward"; }
+};
+
+Tensor dropout(const Tensor &x, double p, const std::optional<Tensor> &rng_, int64_t call) {
+    const Tensor rng = rng_.value_or(Tensor());
+    check_rows("x", x);
+    check_rate(p);
+    check_rng(rng, x);
+    const DropoutArgs args = {p, call};
+    at::Tensor out;
+    {
+        at::NoGradGuard quiet;
+        out = run_dropout(x, args, rng);
+    }
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+        auto node = std::shared_ptr<RofDropoutBackward>(new RofDropoutBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x));
+        node->rng = SavedVariable(rng, false);
+        node->args = args;
+        node->type = x.scalar_type();
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+struct NormArgs {
+    double eps;
+    bool relu;
+    DropoutArgs drop;
+    at::ScalarType out_type;
+};
+
+struct RofLayerNormBackward : public Node {
+    SavedVariable x_, weight_, bias_, rng_;
+    NormArgs args;
+
+    variable_list apply(variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return variable_list(3);
+        const Tensor x = x_.unpack(), weight = weight_.unpack(), bias = bias_.unpack(), rng = rng_.unpack();
+        Tensor dx, dw, db;
+        {
+            at::NoGradGuard quiet;
+            const c10::DeviceGuard guard(x.device());
+            const Tensor grad = gradient_rows(grads[0], args.out_type);
+            const int64_t n = x.size(0), f = x.size(1);
+            const auto floats = x.options().dtype(at::kFloat);
+            if (task_should_compute_output(0)) dx = at::empty({n, f}, x.options());
+            if (task_should_compute_output(1)) dw = at::empty({f}, floats);
+            if (task_should_compute_output(2)) db = at::empty({f}, floats);
+            Tensor workspace;
+            const size_t bytes = dw.defined() || db.defined() ? rof_layer_norm_backward_workspace_bytes(n, (int)f) : 0;
+            if (bytes) workspace = at::empty({(int64_t)(bytes / sizeof(float))}, floats);
+            const rof_dropout_opts opts = {args.drop.p, (const int64_t *)address(rng), args.drop.call};
+            check(rof_layer_norm_backward(grad.data_ptr(), type_of(args.out_type), row_stride(grad), x.data_ptr(),
+                                          type_of(x.scalar_type()), row_stride(x), n, (int)f, (const float *)address(weight),
+                                          (const float *)address(bias), args.eps, args.relu, args.drop.p > 0 ? &opts : nullptr,
+                                          address(dx), f, (float *)address(dw), (float *)address(db), address(workspace), bytes,
+                                          current_stream(x)),
+                  "layer norm's gradient");
+        }
+        return once({dx, dw, db}, "layer_norm");
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        weight_.reset_data();
+        bias_.reset_data();
+        rng_.reset_data();
+    }
+    std::string name() const override { return "RofLayerNormBackward"; }
+};
+
+Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight_, const std::optional<Tensor> &bias_, double eps, bool relu,
+                  double p, const std::optional<Tensor> &rng_, int64_t call, std::optional<at::ScalarType> out_type) {
+    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+    check_rows("x", x);
+    require(x.size(1) <= ROF_LAYER_NORM_MAX_COLUMNS, "layer_norm takes at most 16384 columns");
+    static_assert(ROF_LAYER_NORM_MAX_COLUMNS == 16384, "the message above");
+    check_param("weight", weight, x);
+    check_param("bias", bias, x);
+    require(eps >= 0.0 && eps <= 1e30, "eps must not be negative, and finite");
+    check_rate(p);
+    Tensor rng;
+    if (p > 0) {
+        rng = rng_.value_or(Tensor());
+        check_rng(rng, x);
+    }
+    const NormArgs args = {eps, relu, {p, call}, out_type.value_or(x.scalar_type())};
+    require(known(args.out_type), "out_dtype must be float32 or bfloat16");
+    Tensor out;
+    {
+        at::NoGradGuard quiet;
+        const c10::DeviceGuard guard(x.device());
+        out = at::empty({x.size(0), x.size(1)}, x.options().dtype(args.out_type));
+        const rof_dropout_opts opts = {p, (const int64_t *)address(rng), call};
+        check(rof_layer_norm(x.data_ptr(), type_of(x.scalar_type()), row_stride(x), x.size(0), (int)x.size(1),
+                             (const float *)address(weight), (const float *)address(bias), eps, relu, p > 0 ? &opts : nullptr,
+                             out.data_ptr(), type_of(args.out_type), x.size(1), current_stream(x)),
+              "layer norm");
+    }
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
+        auto node = std::shared_ptr<RofLayerNormBackward>(new RofLayerNormBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+        node->x_ = SavedVariable(x, false);
+        node->weight_ = SavedVariable(weight, false);
+        node->bias_ = SavedVariable(bias, false);
+        node->rng_ = SavedVariable(rng, false);
+        node->args = args;
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+// The values of one step, and the state moved on behind it.
+Tensor dropout_state_next(const Tensor &state, int64_t calls) {
+    require(state.is_cuda(), "the dropout state must be on the GPU (move the module there)");
+    require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous(),
+            "the dropout state must be a contiguous int64 tensor {seed, offset}");
+    require(calls >= 0, "calls must not be negative");
+    const c10::DeviceGuard guard(state.device());
+    Tensor used = at::empty({2}, state.options());
+    check(rof_dropout_state_next((int64_t *)state.data_ptr(), calls, (int64_t *)used.data_ptr(), current_stream(state)),
+          "dropout state");
+    state.unsafeGetTensorImpl()->bump_version();   // a backward pass that kept the state itself has to notice
+    return used;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const Failure &e) {
+            PyErr_SetString(g_error_type ? g_error_type : PyExc_RuntimeError, e.what());
+        }
+    });
+    m.def("set_error_type", [](py::object type) {
+        Py_XDECREF(g_error_type);
+        g_error_type = type.release().ptr();
+    });
+    m.def("layer_norm", &layer_norm, "dropout(relu(layer norm)) of every row (gfx950)");
+    m.def("dropout", &dropout, "dropout without a stored mask (gfx950)");
+    m.def("dropout_state_next", &dropout_state_next, "the values of one step; moves the state on (gfx950)");
+}

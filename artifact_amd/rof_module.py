@@ -18,16 +18,28 @@ from . import _lib
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-def compiled():
-    """The compiled module; raises ImportError naming the build command if it has not been built."""
+def _load(name):
     import torch  # noqa: F401  (the module links against PyTorch's libraries: load them first)
 
     _lib.lib()    # librof.so, with the HIP runtime PyTorch brought
     try:
-        return importlib.import_module("artifact_amd._ROF")
+        return importlib.import_module("artifact_amd." + name)
     except ImportError as ex:
-        raise ImportError(f"artifact_amd/_ROF*.so is not built or does not load ({ex}); run "
+        raise ImportError(f"artifact_amd/{name}*.so is not built or does not load ({ex}); run "
                           f"`python -m artifact_amd.build`") from ex
+
+
+def compiled():
+    """The compiled module; raises ImportError naming the build command if it has not been built."""
+    return _load("_ROF")
+
+
+def row_operators():
+    """The compiled half of artifact_amd.row_ops (`artifact_amd/_ROFrows*.so`, csrc/row_ops_torch.cpp); raises like
+    `compiled`."""
+    mod = _load("_ROFrows")
+    mod.set_error_type(_lib.RofError)
+    return mod
 
 
 def install(name="ROF"):
