@@ -9,72 +9,97 @@ not part of the upstream tree.  The constructor and call conventions are the one
 
 `n_layers` hidden convolutions plus the output convolution, i.e. n_layers + 1 layers (ROF_main.py:256 reports
 "layers": n_layers + 1), activation between them, dropout on the input of every layer but the first.
+
+Both models take two keyword arguments that upstream does not have:
+    norm="layer"        layer norm of every hidden layer's output, before its activation
+    dropout_seed=int    dropout from a counter-based generator whose mask is never stored (row_ops.dropout) in place of
+                        torch.nn.Dropout; the generator's state is a buffer of the model
+With both and a ReLU (or no activation), norm, activation and dropout of a hidden layer are one pass over its rows each way.
 """
 from __future__ import annotations
 
 import torch
 
 from .reuse_conv import ROF_GCNConv, ROF_GINConv, ROF_inputInfo  # noqa: F401  (re-exported like upstream)
+from .row_ops import ROF_Dropout, ROF_DropoutState, ROF_LayerNorm, layer_norm
 
 __all__ = ["ROF_GCN", "ROF_GIN", "ROF_inputInfo"]
+
+_RELUS = (torch.relu, torch.nn.functional.relu)
+
+
+def _add_tails(model, widths, activation, rate, norm, dropout_seed):
+    """What follows the hidden layers of these widths: the model's norms, activation, dropout and dropout state."""
+    if norm not in (None, "layer"):
+        raise ValueError("norm must be None or 'layer'")
+    model.activation = activation
+    model.norms = None if norm is None else torch.nn.ModuleList(ROF_LayerNorm(w) for w in widths)
+    model.dropout = torch.nn.Dropout(p=rate) if dropout_seed is None else ROF_Dropout(rate)
+    model.dropout_state = None if dropout_seed is None else ROF_DropoutState(dropout_seed)
+
+
+def _run_layers(model, h, inputInfo, activated):
+    """The layers and what is between them.  `activated`: the hidden layers apply the activation themselves."""
+    last = len(model.layers) - 1
+    counted = model.dropout_state is not None
+    rate = model.dropout.p if counted and model.dropout.training else 0.0
+    rng = model.dropout_state.next(last) if rate and last else None    # the values of this forward pass
+    dropped = True                                                      # what the next layer reads is ready for it
+    for i, layer in enumerate(model.layers):
+        if not dropped:
+            h = model.dropout(h, rng, call=i - 1) if counted else model.dropout(h)
+        h = layer(h, inputInfo)
+        if i == last:
+            break
+        dropped = False
+        activation = None if activated else model.activation
+        if model.norms is not None:
+            norm, whole = model.norms[i], activation is None or activation in _RELUS
+            dropped = whole and counted
+            h = layer_norm(h, norm.weight, norm.bias, eps=norm.eps, relu=whole and activation is not None,
+                           dropout=rate if dropped else 0.0, rng=rng, call=i)
+            activation = None if whole else activation
+        if activation is not None:
+            h = activation(h)
+    return h
 
 
 class ROF_GCN(torch.nn.Module):
     def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, dropout, add_self_loops=False,
                  reuse_size=0, kernel_type="ROF_v1", bias=True, order="update_first", fuse_epilogue=True,
-                 compute_dtype=None):
+                 compute_dtype=None, norm=None, dropout_seed=None):
         """`order`, `fuse_epilogue` and `compute_dtype` are passed to every ROF_GCNConv (not upstream).  A ReLU
         activation is then applied by the aggregation kernel of each hidden layer rather than as a pass of its
         own.  compute_dtype="bf16": bfloat16 rows and GEMM operands, fp32 sums and parameters; hidden layers hand
-        bfloat16 to each other, the last layer returns float32."""
+        bfloat16 to each other, the last layer returns float32.  `norm`, `dropout_seed`: see the module."""
         super().__init__()
         dims = [in_feats] + [n_hidden] * n_layers + [n_classes]
         last = len(dims) - 2
         bf16 = compute_dtype in ("bf16", torch.bfloat16)
-        self._fused_act = bool(fuse_epilogue) and (kernel_type != "ROF_v1" or bf16) and activation in (
-            torch.relu, torch.nn.functional.relu)
+        self._fused_act = norm is None and bool(fuse_epilogue) and (kernel_type != "ROF_v1" or bf16) and activation in _RELUS
         self.layers = torch.nn.ModuleList(
             ROF_GCNConv(dims[i], dims[i + 1], bias=bias, add_self_loops=add_self_loops, reuse_size=reuse_size,
                         kernel_type=kernel_type, order=order, fuse_epilogue=fuse_epilogue,
                         activation="relu" if self._fused_act and i != last else None, compute_dtype=compute_dtype,
                         out_dtype="bf16" if bf16 and i != last else None)
             for i in range(len(dims) - 1))
-        self.activation = activation
-        self.dropout = torch.nn.Dropout(p=dropout)
+        _add_tails(self, dims[1:-1], activation, dropout, norm, dropout_seed)
 
     def forward(self, features, *args):
-        inputInfo = args[-1]
-        h = features
-        last = len(self.layers) - 1
-        for i, layer in enumerate(self.layers):
-            if i != 0:
-                h = self.dropout(h)
-            h = layer(h, inputInfo)
-            if i != last and self.activation is not None and not self._fused_act:
-                h = self.activation(h)
-        return h
+        return _run_layers(self, features, args[-1], self._fused_act)
 
 
 class ROF_GIN(torch.nn.Module):
-    """GIN with sum aggregation (eps fixed) and one linear map per layer, e.g. 3 x (64 -> 64)."""
+    """GIN with sum aggregation (eps fixed) and one linear map per layer, e.g. 3 x (64 -> 64).  `norm`, `dropout_seed`:
+    see the module."""
 
     def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0, eps=0.0,
-                 kernel_type="ROF_v2"):
+                 kernel_type="ROF_v2", norm=None, dropout_seed=None):
         super().__init__()
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
         self.layers = torch.nn.ModuleList(ROF_GINConv(dims[i], dims[i + 1], eps=eps, kernel_type=kernel_type)
                                           for i in range(len(dims) - 1))
-        self.activation = activation
-        self.dropout = torch.nn.Dropout(p=dropout)
+        _add_tails(self, dims[1:-1], activation, dropout, norm, dropout_seed)
 
     def forward(self, features, *args):
-        inputInfo = args[-1]
-        h = features
-        last = len(self.layers) - 1
-        for i, layer in enumerate(self.layers):
-            if i != 0:
-                h = self.dropout(h)
-            h = layer(h, inputInfo)
-            if i != last and self.activation is not None:
-                h = self.activation(h)
-        return h
+        return _run_layers(self, features, args[-1], False)

@@ -3,6 +3,7 @@ training mask, accuracy on a validation mask) on the synthetic workloads, since 
 (`data_prepare.load_graph`) and its datasets are not available.
 
     python -m artifact_amd.train --workload c1 --epochs 50 --kernel_type ROF_v2
+    python -m artifact_amd.train --workload c1 --norm layer --dropout_seed 7
 """
 from __future__ import annotations
 
@@ -75,6 +76,8 @@ def main():
     ap.add_argument("--epochs", type=int, default=50)
     ap.add_argument("--dim_input", type=int, default=32)
     ap.add_argument("--n_classes", type=int, default=8)
+    ap.add_argument("--norm", default=None, choices=["layer"], help="normalise the hidden layers' outputs")
+    ap.add_argument("--dropout_seed", type=int, default=None, help="dropout from a counter-based generator with this seed")
     args = ap.parse_args()
     dev = torch.device("cuda")
     indptr, indices = make_workload(args.workload, args.scale_down)
@@ -85,7 +88,8 @@ def main():
     split = rng.random(n)
     info = build_input_info(indptr, indices, args.part_size, device=dev)
     model = ROF_GCN(args.dim_input, args.n_hidden, args.n_classes, args.n_layers, F.relu, 0.5, add_self_loops=False,
-                    reuse_size=info.reuse_size, kernel_type=args.kernel_type).to(dev)
+                    reuse_size=info.reuse_size, kernel_type=args.kernel_type, norm=args.norm,
+                    dropout_seed=args.dropout_seed).to(dev)
     feats, labels = torch.from_numpy(x).to(dev), torch.from_numpy(y).to(dev)
     tm, vm, sm = (torch.from_numpy(m).to(dev) for m in (split < 0.6, (split >= 0.6) & (split < 0.8), split >= 0.8))
     losses, accs, dur = train(model, feats, info, labels, tm, vm, args.epochs, log_every=max(1, args.epochs // 10))

@@ -150,3 +150,22 @@ def test_modules_hold_float32_parameters_and_the_generators_state():
     assert s.state_dict()["state"].tolist() == [11, 0] and not list(s.parameters())
     x = torch.zeros(2, 3)
     assert row_ops.ROF_Dropout(0.5).eval()(x, None) is x and row_ops.ROF_Dropout(0.0)(x, None) is x
+
+
+def test_models_take_norm_and_seed():
+    from artifact_amd.ROF_models import ROF_GCN, ROF_GIN
+
+    plain = ROF_GCN(6, 8, 3, 2, torch.relu, 0.5, reuse_size=0)
+    assert not any(k.startswith(("norms", "dropout")) for k in plain.state_dict())
+    for model in (ROF_GCN(6, 8, 3, 2, torch.relu, 0.5, norm="layer", dropout_seed=4),
+                  ROF_GIN(6, 8, 3, 3, dropout=0.5, norm="layer", dropout_seed=4)):
+        keys = {k for k in model.state_dict() if k.startswith(("norms", "dropout"))}
+        assert keys == {"norms.0.weight", "norms.0.bias", "norms.1.weight", "norms.1.bias", "dropout_state.state"}
+        assert isinstance(model.dropout, row_ops.ROF_Dropout) and model.dropout_state.state.tolist() == [4, 0]
+    for bad in ("batch", True, 0):
+        with pytest.raises(ValueError, match="norm"):
+            ROF_GCN(6, 8, 3, 2, torch.relu, 0.5, norm=bad)
+        with pytest.raises(ValueError, match="norm"):
+            ROF_GIN(6, 8, 3, 3, norm=bad)
+    with pytest.raises(RofError, match="rate"):
+        ROF_GCN(6, 8, 3, 2, torch.relu, 1.5, dropout_seed=4)
