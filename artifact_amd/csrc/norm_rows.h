@@ -373,7 +373,6 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
     float most;
     // the dropout's scale is in the parameters: it is positive, so it passes through the ReLU
     const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, most, a.scale), bias(m, a.bias, 0.f, 0.f, bstore, most, a.scale);
-    const Drop drop(a);
     const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
     const int64_t first = Rounds::first<Map::ROWS>(a);
     Rounds go(a, first, Map::ROWS);
@@ -384,6 +383,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
     Cursor<const TX> x((const TX *)a.x, a.ldx, row, a.n);
     Cursor<TY> out((TY *)a.out, a.ldo, row, a.n);
     next.template load<false>(m, x.at);
+    const Drop drop(a);   // read from memory: after the first row is on its way
     for (; go.left > 0; go.next(a, Map::ROWS)) {
         const bool ok = m.slot < go.left, all = go.step + Map::ROWS <= go.left, further = m.slot + go.step < go.left;
         float v[K][V];
@@ -429,17 +429,23 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
 constexpr float kBorder = 7.62939453125e-06f;
 constexpr float kFarMean = 1024.f;
 
-// The exact sign of pre, in place of its value.  Rare, so it is kept small: it reads the row again.
-template <typename Map, typename TX>
-__device__ __forceinline__ void gate64(const Map &m, const NormArgs &a, const TX *row, bool ok, double (*part)[Map::WAVES_][2], int &turn,
-                                       float (&pre)[Map::K_][Map::V]) {
+// The exact sign of pre, in place of its value.  Rare, so it is kept out of the registers of the common path: the row is read
+// again, a vector at a time.  Not slow either: on a small graph one wavefront that comes here is what the launch waits for.
+template <typename Map, typename TX, typename W, typename B>
+__device__ __forceinline__ void gate64(const Map &m, const NormArgs &a, const TX *row, const W &weight, const B &bias,
+                                       double (*part)[Map::WAVES_][2], int &turn, float (&pre)[Map::K_][Map::V]) {
     constexpr int V = Map::V, K = Map::K_;
-    auto at = [&](int j, float (&v)[V]) {
-        const int count = !ok ? 0 : j < K - 1 ? V : m.last;
+    auto at = [&](int j, float (&v)[V]) {   // columns that do not exist are zero
         Packed<TX, V> p;
-        p.load_few(row + m.col(j), count);
+        if constexpr (Map::LANES == 1) {
+            p.load_few(row, m.last);
+        } else {
+            p.load(row + (j < K - 1 ? m.col(j) : m.from));
+            if (j == K - 1 && m.tail) p.shift(m.back);
+        }
         p.unpack(v);
-        return count;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = m.has(j, e) ? v[e] : 0.f;
     };
     float v[V];
     double s = 0.0, none = 0.0;
@@ -454,32 +460,25 @@ __device__ __forceinline__ void gate64(const Map &m, const NormArgs &a, const TX
     s = none = 0.0;
 #pragma unroll 1
     for (int j = 0; j < K; ++j) {
-        const int count = at(j, v);
+        at(j, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const double c = e < count ? (double)v[e] - mean : 0.0;
+            const double c = m.has(j, e) ? (double)v[e] - mean : 0.0;
             s = fma(c, c, s);
         }
     }
     m.sum2(s, none, part, turn);
     const double r = 1.0 / sqrt(s / a.f + a.eps);
-    uint32_t gate = 0;
-#pragma unroll 1
+#pragma unroll
     for (int j = 0; j < K; ++j) {
-        const int count = at(j, v);
+        float w[V], b[V];
+        at(j, v);
+        weight.get(j, w);
+        bias.get(j, b);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (e < count) {
-                const int c = m.col(j) + e;
-                const double w = a.weight ? (double)a.weight[c] : 1.0, b = a.bias ? (double)a.bias[c] : 0.0;
-                gate |= (fma(((double)v[e] - mean) * r, w, b) > 0.0 ? 1u : 0u) << (j * V + e);
-            }
-        }
+        for (int e = 0; e < V; ++e) pre[j][e] = fma(((double)v[e] - mean) * r, (double)w[e], (double)b[e]) > 0.0 ? 1.f : 0.f;
+        asm volatile("" ::: "memory");   // one vector after the other
     }
-#pragma unroll
-    for (int j = 0; j < K; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) pre[j][e] = (gate >> (j * V + e) & 1u) ? 1.f : 0.f;
 }
 
 // nothing, where the bias is not needed (without a ReLU the gradient does not depend on it)
@@ -507,7 +506,6 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
     for (int j = 0; j < K; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.f;
-    const Drop drop(a);
     const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
     const int64_t first = Rounds::first<Map::ROWS>(a);
     Rounds go(a, first, Map::ROWS);
@@ -521,6 +519,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
     Cursor<TX> dx((TX *)a.out, a.ldo, row, a.n);
     next_x.template load<STREAM>(m, x.at);
     next_d.template load<STREAM>(m, dout.at);
+    const Drop drop(a);   // read from memory: after the first row is on its way
     for (; go.left > 0; go.next(a, Map::ROWS)) {
         const bool ok = m.slot < go.left, all = go.step + Map::ROWS <= go.left, further = m.slot + go.step < go.left;
         float h[K][V], d[K][V];
@@ -569,7 +568,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
             }
             const float far = r * fabsf(mean);
             const bool close = ok && (far > kFarMean || least <= kBorder * fmaf(fmaf(2.f, far, 1.f), wmost, 2.f * bmost));
-            if (WAVES > 1 ? __syncthreads_or(close) : __any(close)) gate64(m, a, here, ok, sh.part64, turn64, pre);
+            if (WAVES > 1 ? __syncthreads_or(close) : __any(close)) gate64(m, a, here, weight, bias, sh.part64, turn64, pre);
 #pragma unroll
             for (int j = 0; j < K; ++j)
 #pragma unroll
@@ -655,7 +654,6 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 // (V(lanes, wavefronts, vectors); STREAMED: those that also exist with streaming accesses.)
 #define ROF_NORM_STREAMED(V) V(8, 1, 1) V(16, 1, 1) V(32, 1, 1) V(64, 1, 1) V(64, 1, 2) V(64, 2, 2) V(64, 4, 2) V(64, 8, 2)
 #define ROF_NORM_OTHERS(V) V(1, 1, 1) V(2, 1, 1) V(4, 1, 1) V(64, 1, 3) V(64, 4, 3) V(64, 8, 3) V(64, 8, 4)
-#define ROF_NORM_F32_ONLY(V) V(64, 16, 3) V(64, 16, 4)   // 16384 bfloat16 columns are 2048 vectors
 
 template <typename TX, typename TY>
 int launch_norm_forward(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {
@@ -668,9 +666,6 @@ int launch_norm_forward(const NormArgs &a, const NormShape &s, int blocks, hipSt
     }
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
     ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
-    if constexpr (sizeof(TX) == 4) {
-        ROF_NORM_F32_ONLY(ROF_NORM_LAUNCH)
-    }
 #undef ROF_NORM_LAUNCH
     return ROF_ERR_UNSUPPORTED;
 }
@@ -689,9 +684,6 @@ int launch_norm_backward(const NormArgs &a, const NormShape &s, int blocks, hipS
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH_STREAMED)
     ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
-    if constexpr (sizeof(TX) == 4) {
-        ROF_NORM_F32_ONLY(ROF_NORM_LAUNCH)
-    }
 #undef ROF_NORM_LAUNCH_STREAMED
 #undef ROF_NORM_LAUNCH
 #undef ROF_NORM_LAUNCH_AS

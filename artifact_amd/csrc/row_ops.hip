@@ -13,7 +13,6 @@ namespace {
 
 using namespace rofn;
 
-constexpr int kMaxNormColumns = ROF_LAYER_NORM_MAX_COLUMNS;
 // Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.  Where there
 // are more rounds of work than kManyRounds it is tiles of eight rounds, see norm_blocks, else workgroups that stay.
 constexpr int kBackwardBlocks = 1024, kBackwardTiles = 16384;
@@ -168,9 +167,11 @@ float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (
 // others twice per row (2048 bfloat16 columns, 256 vectors, 80 M elements: one wavefront with four vectors 57 / 95, two with
 // two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90).
 NormShape norm_shape(int f, int x_dtype) {
+    // every vector of a lane but its last is whole: more than (k - 1) lpr waves of them, which is the row before's `most`
     static const struct { int most, lpr, waves, k; } kShapes[] = {
-        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},     {16, 16, 1, 1},   {32, 32, 1, 1},   {64, 64, 1, 1},  {128, 64, 1, 2},
-        {192, 64, 1, 3}, {256, 64, 2, 2}, {512, 64, 4, 2}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}, {3072, 64, 16, 3}, {4096, 64, 16, 4}};
+        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},    {16, 16, 1, 1},   {32, 32, 1, 1},   {64, 64, 1, 1},
+        {128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2}, {512, 64, 4, 2}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3},
+        {2048, 64, 8, 4}};
     const int vecs = (f * size_of(x_dtype) + 15) / 16;
     NormShape s = {0, 0, 0, false};
     for (const auto &c : kShapes)
@@ -238,7 +239,8 @@ int launch_norm_backward(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st, 
 int norm_args(NormArgs &a, const void *x, int x_dtype, int64_t ldx, int64_t n, int f, const float *weight, const float *bias,
               double eps, int relu, const rof_dropout_opts *dropout, int y_dtype) {
     if (n < 0 || f < 1 || ldx < f || (n && !x) || !(eps >= 0.0 && eps <= 1e30)) return ROF_ERR_ARG;
-    if (!known_type(x_dtype) || !known_type(y_dtype) || f > kMaxNormColumns) return ROF_ERR_UNSUPPORTED;
+    if (!known_type(x_dtype) || !known_type(y_dtype) || f > ROF_LAYER_NORM_MAX_ROW_BYTES / size_of(x_dtype))
+        return ROF_ERR_UNSUPPORTED;
     if (!aligned(x, size_of(x_dtype)) || !aligned(weight, 4) || !aligned(bias, 4)) return ROF_ERR_ARG;
     a = NormArgs();
     a.x = x;

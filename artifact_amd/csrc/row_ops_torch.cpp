@@ -63,6 +63,7 @@ void check_rows(const char *name, const Tensor &t) {
     require(t.is_cuda() && t.dim() == 2 && known(t.scalar_type()), name, " must be a 2-D float32 or bfloat16 CUDA tensor");
     require(t.size(1) > 0 && t.size(1) <= INT32_MAX, name, " must have at least one column");
     require(rows_apart(t), name, " must have unit column stride and rows that do not overlap");
+    require(!t._fw_grad(0).defined(), name, " must not carry a forward-mode tangent (there is no forward-mode derivative)");
 }
 void check_param(const char *name, const Tensor &t, const Tensor &x) {
     require(!t.defined() || (t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 1 &&
@@ -206,8 +207,9 @@ Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight_, const s
                   double p, const std::optional<Tensor> &rng_, int64_t call, std::optional<at::ScalarType> out_type) {
     const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
     check_rows("x", x);
-    require(x.size(1) <= ROF_LAYER_NORM_MAX_COLUMNS, "layer_norm takes at most 16384 columns");
-    static_assert(ROF_LAYER_NORM_MAX_COLUMNS == 16384, "the message above");
+    require(x.size(1) * (int64_t)x.element_size() <= ROF_LAYER_NORM_MAX_ROW_BYTES,
+            "layer_norm takes rows of at most 32768 bytes (8192 float32 or 16384 bfloat16 columns)");
+    static_assert(ROF_LAYER_NORM_MAX_ROW_BYTES == 32768, "the message above");
     check_param("weight", weight, x);
     check_param("bias", bias, x);
     require(eps >= 0.0 && eps <= 1e30, "eps must not be negative, and finite");

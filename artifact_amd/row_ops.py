@@ -14,7 +14,6 @@ from ._lib import RofError
 
 __all__ = ["layer_norm", "dropout", "ROF_LayerNorm", "ROF_Dropout", "ROF_DropoutState"]
 
-LAYER_NORM_MAX_COLUMNS = 16384   # ROF_LAYER_NORM_MAX_COLUMNS of include/rof.h
 _ops = None
 
 
@@ -39,8 +38,8 @@ def dropout(x, p, rng, call=0):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, dropout=0.0, rng=None, call=0, out_dtype=None):
     """dropout(relu(layer norm of every row of x)) in one pass each way.
 
-    x: [n, f] float32 or bfloat16 with unit column stride (rows may be apart), f <= 16384; weight, bias: float32 [f] or
-    None (1 and 0); `relu` and `dropout` (a rate; rng and call as in `dropout`) are left out by default; out_dtype: float32
+    x: [n, f] float32 or bfloat16 with unit column stride (rows may be apart), f <= 8192 or 16384; weight, bias: float32 [f]
+    or None (1 and 0); `relu` and `dropout` (a rate; rng and call as in `dropout`) are left out by default; out_dtype: float32
     or bfloat16, by default x's.  Sums are taken in float32 and the result is rounded once.  The backward pass keeps x only
     and computes statistics, gate and mask from it again; its sums over rows have a fixed order, so the gradients are
     bitwise repeatable.  There is no second derivative.  Raises RofError for what it does not take."""

@@ -75,7 +75,8 @@ def check_norm(x, w, b, dy, relu=False, p=0.0, call=0, out_dtype=None, eps=1e-5)
 SHAPES = [(1, 1), (3, 2), (2, 3), (5, 4), (64, 5), (130, 8), (7, 9), (33, 15), (257, 16), (19, 17), (65, 31), (16, 32), (70, 33),
           (50, 47), (21, 63), (100, 64), (35, 65), (33, 100), (41, 127), (18, 128), (11, 129), (64, 255), (40, 256), (17, 257),
           (9, 511), (7, 513), (6, 1000), (9, 1024), (6, 1025), (5, 2047), (5, 2048), (6, 2049), (4, 4096), (4, 4097), (3, 8191),
-          (2, 8193), (3, 12289), (2, 16384)]
+          (2, 8192), (3, 6145)]
+WIDE = [(2, 8193), (3, 12289), (2, 16384)]          # bfloat16 only: rows of at most 32 KB
 
 
 @pytest.mark.parametrize("xt,yt", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float32", "bfloat16"), ("bfloat16", "float32")])
@@ -91,6 +92,14 @@ def test_layer_norm_and_its_gradient(n, f, xt, yt):
 def test_the_tail_of_a_hidden_layer_and_its_gradient(n, f, xt, yt, relu, p):
     w, b = params(f, f + 7)
     check_norm(rows_of(n, f, xt, n + f), w, b, rows_of(n, f, yt, n + f + 1), relu, p, call=3, out_dtype=TYPES[yt])
+
+
+@pytest.mark.parametrize("yt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,f", WIDE)
+@pytest.mark.parametrize("relu,p", [(False, 0.0), (True, 0.5)])
+def test_the_widest_rows(n, f, yt, relu, p):
+    w, b = params(f, f)
+    check_norm(rows_of(n, f, "bfloat16", n + f), w, b, rows_of(n, f, yt, n + f + 1), relu, p, out_dtype=TYPES[yt])
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
@@ -499,8 +508,14 @@ def test_refusals():
             layer_norm(x, eps=bad)
     with pytest.raises(RofError, match="out_dtype"):
         layer_norm(x, out_dtype=torch.float16)
-    with pytest.raises(RofError, match="at most"):
-        layer_norm(torch.zeros(1, 16385, device="cuda"))
+    for bad in (torch.zeros(1, 8193, device="cuda"), torch.zeros(1, 16385, dtype=torch.bfloat16, device="cuda")):
+        with pytest.raises(RofError, match="at most"):
+            layer_norm(bad)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: layer_norm(dual), lambda: dropout(dual, 0.5, rng)):
+            with pytest.raises(RofError, match="forward-mode"):
+                call()
     y = layer_norm(x.requires_grad_(True))
     g, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
     with pytest.raises(RuntimeError):                              # no second derivative

@@ -73,7 +73,8 @@ def _norm(x=PTR, xt=F32, ldx=8, n=3, f=8, w=PTR, b=PTR, eps=1e-5, drop=None, out
 @pytest.mark.parametrize("args,code", [
     (dict(n=-1), ARG), (dict(f=0, ldx=0), ARG), (dict(ldx=7), ARG), (dict(ldo=7), ARG), (dict(x=None), ARG),
     (dict(out=None), ARG), (dict(eps=-1.0), ARG), (dict(eps=float("nan")), ARG), (dict(eps=float("inf")), ARG),
-    (dict(xt=2), UNSUPPORTED), (dict(ot=-1), UNSUPPORTED), (dict(f=16385, ldx=16385, ldo=16385), UNSUPPORTED),
+    (dict(xt=2), UNSUPPORTED), (dict(ot=-1), UNSUPPORTED), (dict(f=8193, ldx=8193, ldo=8193), UNSUPPORTED),
+    (dict(xt=BF16, f=16385, ldx=16385, ldo=16385), UNSUPPORTED),
     (dict(x=PTR + 2), ARG), (dict(xt=BF16, x=PTR + 1), ARG), (dict(w=PTR + 2), ARG), (dict(b=PTR + 1), ARG),
     (dict(out=PTR + 2), ARG), (dict(ot=BF16, out=PTR + 1), ARG),
     (dict(drop=DropoutOpts(-0.1, PTR, 0)), ARG), (dict(drop=DropoutOpts(1.5, PTR, 0)), ARG),
@@ -89,7 +90,7 @@ def test_layer_norm_refuses_what_it_cannot_run(args, code):
 @pytest.mark.parametrize("args,code", [
     (dict(dout=None), ARG), (dict(ldd=7), ARG), (dict(dout=PTR + 2), ARG), (dict(lddx=7), ARG), (dict(dx=PTR + 1), ARG),
     (dict(dw=PTR + 2), ARG), (dict(db=PTR + 2), ARG), (dict(ws=None), WORKSPACE), (dict(size=3 * 2 * 8 * 4 - 1), WORKSPACE),
-    (dict(ws=PTR + 8), WORKSPACE), (dict(f=16385, ldx=16385), UNSUPPORTED), (dict(dt=7), UNSUPPORTED), (dict(n=-1), ARG),
+    (dict(ws=PTR + 8), WORKSPACE), (dict(f=8193, ldx=8193), UNSUPPORTED), (dict(dt=7), UNSUPPORTED), (dict(n=-1), ARG),
     (dict(dx=None, dw=None, db=None, ws=None, size=0), 0),      # nothing wanted: nothing launched
 ])
 def test_layer_norm_backward_refuses_what_it_cannot_run(args, code):
