@@ -165,13 +165,14 @@ float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (
 //   2^18 x 256 float32, 64 vectors: 64 lanes 105 / 165, 32 lanes with two vectors 104 / 173.
 // Above that two or three vectors per lane and as few wavefronts as that takes, because every wavefront more waits for the
 // others twice per row (2048 bfloat16 columns, 256 vectors, 80 M elements: one wavefront with four vectors 57 / 95, two with
-// two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90).
+// two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90), and as few idle lanes
+// (20011 x 4099 bfloat16, 513 vectors: three with three 62 / 115, four with three 72 / 119, eight with two 88 / 160).
 NormShape norm_shape(int f, int x_dtype) {
-    // every vector of a lane but its last is whole: more than (k - 1) lpr waves of them, which is the row before's `most`
+    // every vector of a lane but its last is whole, because the row before's `most` is at least (k - 1) lpr waves
     static const struct { int most, lpr, waves, k; } kShapes[] = {
-        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},    {16, 16, 1, 1},   {32, 32, 1, 1},   {64, 64, 1, 1},
-        {128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2}, {512, 64, 4, 2}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3},
-        {2048, 64, 8, 4}};
+        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},    {16, 16, 1, 1},   {32, 32, 1, 1},
+        {64, 64, 1, 1},  {128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2}, {384, 64, 3, 2},  {512, 64, 4, 2},
+        {576, 64, 3, 3}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}};
     const int vecs = (f * size_of(x_dtype) + 15) / 16;
     NormShape s = {0, 0, 0, false};
     for (const auto &c : kShapes)
@@ -181,12 +182,13 @@ NormShape norm_shape(int f, int x_dtype) {
 
 // How many workgroups, and which rounds each takes.
 // Forward: a workgroup per four adjacent rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
-// with 2048 workgroups that stay and step through the matrix together; 10^6 x 100 float32 142 / 155), else as many as stay.
+// with 2048 workgroups that stay and step through the matrix together; 10^6 x 100 float32 142 / 155), else as many as stay:
+// 2048, or half as many where the lanes hold several vectors.
 // Backward: each workgroup leaves a row of partial sums.  With many rounds it is up to 16384 tiles of eight adjacent ones,
 // handed out as others end (2^22 x 256 bfloat16: 1221 us against 1355 with 1024 workgroups that stay, 2.4 M x 47 float32
 // 258 / 285, 10^6 x 100 233 / 272); with fewer 1024 that stay (2^20 x 64 bfloat16: 66 / 73), half as many where the lanes
-// hold several vectors, whose registers leave room for no more, and two adjacent rounds at a time (20011 x 4099 bfloat16:
-// 106 us against 117 one at a time; forward 73 / 80).
+// hold several vectors, whose registers leave room for no more, and two adjacent rounds at a time (20011 x 4099 bfloat16
+// with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
 int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
     const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
     const bool lean = s.waves == 1 && s.k == 1;
@@ -199,7 +201,7 @@ int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
         most = kBackwardTiles;
     } else {
         a.inner = lean || rounds < 2048 ? 1 : 2;
-        most = backward ? (lean || s.waves == 2 ? kBackwardBlocks : kBackwardBlocks / 2) : 2048;
+        most = backward ? (lean || s.waves == 2 ? kBackwardBlocks : kBackwardBlocks / 2) : lean ? 2048 : 1024;
     }
     const int blocks = (int)std::min<int64_t>((rounds + a.inner - 1) / a.inner, most);
     a.jump = ((int64_t)blocks * a.inner - (a.inner - 1)) * rows;

@@ -74,8 +74,8 @@ def check_norm(x, w, b, dy, relu=False, p=0.0, call=0, out_dtype=None, eps=1e-5)
 # a row per lane group, per wavefront, per four and per sixteen of them, each at its borders; odd numbers of rows and columns
 SHAPES = [(1, 1), (3, 2), (2, 3), (5, 4), (64, 5), (130, 8), (7, 9), (33, 15), (257, 16), (19, 17), (65, 31), (16, 32), (70, 33),
           (50, 47), (21, 63), (100, 64), (35, 65), (33, 100), (41, 127), (18, 128), (11, 129), (64, 255), (40, 256), (17, 257),
-          (9, 511), (7, 513), (6, 1000), (9, 1024), (6, 1025), (5, 2047), (5, 2048), (6, 2049), (4, 4096), (4, 4097), (3, 8191),
-          (2, 8192), (3, 6145)]
+          (9, 511), (7, 513), (6, 1000), (9, 1024), (6, 1025), (5, 2047), (5, 2048), (6, 2049), (4, 4096), (4, 4097), (3, 4608), (3, 4609), (3, 8191),
+          (2, 8192), (3, 6145), (9, 1537), (9, 1536), (9, 2304), (9, 2305)]
 WIDE = [(2, 8193), (3, 12289), (2, 16384)]          # bfloat16 only: rows of at most 32 KB
 
 
