@@ -651,8 +651,10 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 
 // ---- launch ---------------------------------------------------------------------------------------------------------
 // The variants that norm_shape (row_ops.hip) chooses among: lanes of a wavefront, wavefronts and vectors per lane.
-// (V(lanes, wavefronts, vectors); STREAMED: those that also exist with streaming accesses.)
+// (V(lanes, wavefronts, vectors); STREAMED: those that also exist with streaming accesses; F32, BF16: for rows of that type.)
 #define ROF_NORM_STREAMED(V) V(8, 1, 1) V(16, 1, 1) V(32, 1, 1) V(64, 1, 1) V(64, 1, 2) V(64, 2, 2) V(64, 3, 2) V(64, 4, 2) V(64, 8, 2)
+#define ROF_NORM_F32(V) V(8, 1, 2) V(16, 1, 2) V(32, 1, 2)
+#define ROF_NORM_BF16(V) V(4, 1, 3) V(8, 1, 3) V(16, 1, 3)
 #define ROF_NORM_OTHERS(V) V(1, 1, 1) V(2, 1, 1) V(4, 1, 1) V(64, 1, 3) V(64, 3, 3) V(64, 4, 3) V(64, 8, 3) V(64, 8, 4)
 
 template <typename TX, typename TY>
@@ -666,6 +668,11 @@ int launch_norm_forward(const NormArgs &a, const NormShape &s, int blocks, hipSt
     }
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
     ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
+    if constexpr (sizeof(TX) == 4) {
+        ROF_NORM_F32(ROF_NORM_LAUNCH)
+    } else {
+        ROF_NORM_BF16(ROF_NORM_LAUNCH)
+    }
 #undef ROF_NORM_LAUNCH
     return ROF_ERR_UNSUPPORTED;
 }
@@ -684,6 +691,11 @@ int launch_norm_backward(const NormArgs &a, const NormShape &s, int blocks, hipS
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH)
     ROF_NORM_STREAMED(ROF_NORM_LAUNCH_STREAMED)
     ROF_NORM_OTHERS(ROF_NORM_LAUNCH)
+    if constexpr (sizeof(TX) == 4) {
+        ROF_NORM_F32(ROF_NORM_LAUNCH)
+    } else {
+        ROF_NORM_BF16(ROF_NORM_LAUNCH)
+    }
 #undef ROF_NORM_LAUNCH_STREAMED
 #undef ROF_NORM_LAUNCH
 #undef ROF_NORM_LAUNCH_AS

@@ -17,7 +17,7 @@ using namespace rofn;
 // are more rounds of work than kManyRounds it is tiles of eight rounds, see norm_blocks, else workgroups that stay.
 constexpr int kBackwardBlocks = 1024, kBackwardTiles = 16384;
 constexpr int64_t kManyRounds = 65536;
-constexpr int kTiledColumns = 512;   // rows of more columns are several vectors per lane in either type
+constexpr int kTiledColumns = 512;   // rows of more columns are several vectors per lane of a whole wavefront in either type
 constexpr int kParamsChunks = 128;   // rows that the first of two passes leaves of so many partial ones
 // An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
 constexpr int64_t kStreamOutBytes = 128 << 20;
@@ -163,21 +163,27 @@ float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (
 // that holds it: few registers, and the rows of a wavefront are one contiguous piece.  Measured (us, forward / backward):
 //   2^20 x 64 bfloat16, 8 vectors: 8 lanes 41 / 66, 4 lanes with two vectors 40 / 79, 16 lanes half empty 53 / 97;
 //   2^18 x 256 float32, 64 vectors: 64 lanes 105 / 165, 32 lanes with two vectors 104 / 173.
+// A group of 16 or more lanes of which that would leave a quarter idle is half as many lanes with two vectors (float32) or a
+// quarter with three (bfloat16, whose arithmetic per byte is twice as much); with ReLU and dropout:
+//   667 000 x 150 float32, 38 vectors: 32 lanes with two 151 / 242, 64 lanes 188 / 288, 16 with three 152 / 247;
+//   667 000 x 300 bfloat16, 38 vectors: 16 lanes with three 153 / 286, 64 lanes 235 / 372, 32 with two 181 / 393.
 // Above that two or three vectors per lane and as few wavefronts as that takes, because every wavefront more waits for the
 // others twice per row (2048 bfloat16 columns, 256 vectors, 80 M elements: one wavefront with four vectors 57 / 95, two with
 // two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90), and as few idle lanes
 // (20011 x 4099 bfloat16, 513 vectors: three with three 62 / 115, four with three 72 / 119, eight with two 88 / 160).
 NormShape norm_shape(int f, int x_dtype) {
-    // every vector of a lane but its last is whole, because the row before's `most` is at least (k - 1) lpr waves
-    static const struct { int most, lpr, waves, k; } kShapes[] = {
-        {1, 1, 1, 1},    {2, 2, 1, 1},    {4, 4, 1, 1},    {8, 8, 1, 1},    {16, 16, 1, 1},   {32, 32, 1, 1},
-        {64, 64, 1, 1},  {128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2}, {384, 64, 3, 2},  {512, 64, 4, 2},
-        {576, 64, 3, 3}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}};
+    // In every entry the vectors of a lane but its last are whole, because the entry before it ends at (k - 1) lpr waves or later.
+    struct Shape { int most, lpr, waves, k; };
+    static const Shape kF32[] = {{1, 1, 1, 1},   {2, 2, 1, 1},   {4, 4, 1, 1},   {8, 8, 1, 1},   {11, 8, 1, 2}, {16, 16, 1, 1},
+                                 {23, 16, 1, 2}, {32, 32, 1, 1}, {47, 32, 1, 2}, {64, 64, 1, 1}};
+    static const Shape kBf16[] = {{1, 1, 1, 1},  {2, 2, 1, 1},   {4, 4, 1, 1},   {8, 8, 1, 1},  {12, 4, 1, 3}, {16, 16, 1, 1},
+                                  {24, 8, 1, 3}, {32, 32, 1, 1}, {48, 16, 1, 3}, {64, 64, 1, 1}};
+    static const Shape kWide[] = {{128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2},  {384, 64, 3, 2},  {512, 64, 4, 2},
+                                  {576, 64, 3, 3}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}};
     const int vecs = (f * size_of(x_dtype) + 15) / 16;
-    NormShape s = {0, 0, 0, false};
-    for (const auto &c : kShapes)
-        if (!s.k && vecs <= c.most) s = {c.lpr, c.waves, c.k, false};
-    return s;
+    const Shape *c = vecs > 64 ? kWide : x_dtype == ROF_F32 ? kF32 : kBf16;
+    while (vecs > c->most) ++c;   // ends: a row is at most 2048 vectors
+    return {c->lpr, c->waves, c->k, false};
 }
 
 // How many workgroups, and which rounds each takes.
@@ -191,7 +197,7 @@ NormShape norm_shape(int f, int x_dtype) {
 // with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
 int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
     const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
-    const bool lean = s.waves == 1 && s.k == 1;
+    const bool lean = s.waves == 1 && (s.k == 1 || s.lpr < 64);
     int64_t most;
     if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
         a.inner = 4;
@@ -213,7 +219,7 @@ int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
 // 2^20 x 64 bfloat16 66 / 74; rows of 47 columns, whose lines two wavefronts share, 288 / 258).
 bool norm_streams(const NormArgs &a, const NormShape &s, int x_dtype, int y_dtype) {
     const int sx = size_of(x_dtype), sy = size_of(y_dtype);
-    if (a.n * a.f * sx < kStreamOutBytes || s.k > 2 || s.lpr < 8) return false;
+    if (a.n * a.f * sx < kStreamOutBytes || s.k > 2 || s.lpr < 8 || (s.k > 1 && s.lpr < 64)) return false;
     return aligned(a.x, 16) && aligned(a.dout, 16) && aligned(a.out, 16) && a.ldx * sx % 16 == 0 && a.ldd * sy % 16 == 0 &&
            a.ldo * sx % 16 == 0 && (int64_t)a.f * sx % 16 == 0;
 }
