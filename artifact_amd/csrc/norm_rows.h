@@ -655,7 +655,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 #define ROF_NORM_STREAMED(V) V(8, 1, 1) V(16, 1, 1) V(32, 1, 1) V(64, 1, 1) V(64, 1, 2) V(64, 2, 2) V(64, 3, 2) V(64, 4, 2) V(64, 8, 2)
 #define ROF_NORM_F32(V) V(8, 1, 2) V(16, 1, 2) V(32, 1, 2)
 #define ROF_NORM_BF16(V) V(4, 1, 3) V(8, 1, 3) V(16, 1, 3)
-#define ROF_NORM_OTHERS(V) V(1, 1, 1) V(2, 1, 1) V(4, 1, 1) V(64, 1, 3) V(64, 3, 3) V(64, 4, 3) V(64, 8, 3) V(64, 8, 4)
+#define ROF_NORM_OTHERS(V) V(1, 1, 1) V(2, 1, 1) V(4, 1, 1) V(32, 1, 3) V(64, 1, 3) V(64, 3, 3) V(64, 4, 3) V(64, 8, 3) V(64, 8, 4)
 
 template <typename TX, typename TY>
 int launch_norm_forward(const NormArgs &a, const NormShape &s, int blocks, hipStream_t st) {

@@ -160,17 +160,21 @@ int drop_threshold(const rof_dropout_opts *d) {
 float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.f; }
 
 // The variant for f columns.  A row of up to 64 vectors of 16 bytes is one vector in each lane of the smallest lane group
-// that holds it: few registers, and the rows of a wavefront are one contiguous piece.  Measured (us, forward / backward):
-//   2^20 x 64 bfloat16, 8 vectors: 8 lanes 41 / 66, 4 lanes with two vectors 40 / 79, 16 lanes half empty 53 / 97;
-//   2^18 x 256 float32, 64 vectors: 64 lanes 105 / 165, 32 lanes with two vectors 104 / 173.
+// that holds it: few registers, and the rows of a wavefront are one contiguous piece.  Measured (us, forward / backward, each
+// with the launch size that suits it best):
+//   2^20 x 64 bfloat16, 8 vectors: 8 lanes 40 / 70, 4 lanes with two vectors 39 / 75, 16 lanes half empty 50 / 96;
+//   2^22 x 256 bfloat16, 32 vectors, with ReLU and dropout: 32 lanes 742 / 1125, 16 with two 736 / 1194;
+//   2^18 x 256 float32, 64 vectors: 64 lanes 92 / 134, 32 lanes with two vectors 92 / 131.
 // A group of 16 or more lanes of which that would leave a quarter idle is half as many lanes with two vectors (float32) or a
 // quarter with three (bfloat16, whose arithmetic per byte is twice as much); with ReLU and dropout:
-//   667 000 x 150 float32, 38 vectors: 32 lanes with two 151 / 242, 64 lanes 188 / 288, 16 with three 152 / 247;
-//   667 000 x 300 bfloat16, 38 vectors: 16 lanes with three 153 / 286, 64 lanes 235 / 372, 32 with two 181 / 393.
+//   667 000 x 150 float32, 38 vectors: 32 lanes with two 147 / 240, 64 lanes 173 / 277, 16 with three 147 / 242;
+//   667 000 x 300 bfloat16, 38 vectors: 16 lanes with three 153 / 261, 64 lanes 213 / 348, 32 with two 177 / 339.
 // Above that two or three vectors per lane and as few wavefronts as that takes, because every wavefront more waits for the
-// others twice per row (2048 bfloat16 columns, 256 vectors, 80 M elements: one wavefront with four vectors 57 / 95, two with
-// two 55 / 78, four with one 60 / 87; 8192 columns: four with four 58 / 102, eight with two 54 / 90), and as few idle lanes
-// (20011 x 4099 bfloat16, 513 vectors: three with three 62 / 115, four with three 72 / 119, eight with two 88 / 160).
+// others twice per row, and as few idle lanes; bfloat16:
+//   385 000 x 520, 65 vectors, with ReLU and dropout: 32 lanes with three 153 / 271, 64 with two 186 / 356;
+//   39 000 x 2048, 256 vectors: two wavefronts with two vectors 57 / 83, one with four 54 / 93, four with one 56 / 83;
+//   20011 x 4099, 513 vectors: three with three 62 / 112, four with three 78 / 117, eight with two 89 / 159;
+//   9765 x 8192, 1024 vectors: eight with two 54 / 86, four with four 55 / 98.
 NormShape norm_shape(int f, int x_dtype) {
     // In every entry the vectors of a lane but its last are whole, because the entry before it ends at (k - 1) lpr waves or later.
     struct Shape { int most, lpr, waves, k; };
@@ -178,7 +182,7 @@ NormShape norm_shape(int f, int x_dtype) {
                                  {23, 16, 1, 2}, {32, 32, 1, 1}, {47, 32, 1, 2}, {64, 64, 1, 1}};
     static const Shape kBf16[] = {{1, 1, 1, 1},  {2, 2, 1, 1},   {4, 4, 1, 1},   {8, 8, 1, 1},  {12, 4, 1, 3}, {16, 16, 1, 1},
                                   {24, 8, 1, 3}, {32, 32, 1, 1}, {48, 16, 1, 3}, {64, 64, 1, 1}};
-    static const Shape kWide[] = {{128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2},  {384, 64, 3, 2},  {512, 64, 4, 2},
+    static const Shape kWide[] = {{96, 32, 1, 3},  {128, 64, 1, 2}, {192, 64, 1, 3}, {256, 64, 2, 2},  {384, 64, 3, 2}, {512, 64, 4, 2},
                                   {576, 64, 3, 3}, {768, 64, 4, 3}, {1024, 64, 8, 2}, {1536, 64, 8, 3}, {2048, 64, 8, 4}};
     const int vecs = (f * size_of(x_dtype) + 15) / 16;
     const Shape *c = vecs > 64 ? kWide : x_dtype == ROF_F32 ? kF32 : kBf16;
@@ -197,7 +201,7 @@ NormShape norm_shape(int f, int x_dtype) {
 // with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
 int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
     const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
-    const bool lean = s.waves == 1 && (s.k == 1 || s.lpr < 64);
+    const bool lean = s.waves * s.lpr * s.k <= 64;   // rows of up to 64 vectors: kTiledColumns
     int64_t most;
     if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
         a.inner = 4;
@@ -207,7 +211,7 @@ int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
         most = kBackwardTiles;
     } else {
         a.inner = lean || rounds < 2048 ? 1 : 2;
-        most = backward ? (lean || s.waves == 2 ? kBackwardBlocks : kBackwardBlocks / 2) : lean ? 2048 : 1024;
+        most = backward ? (lean || s.waves == 2 || s.lpr < 64 ? kBackwardBlocks : kBackwardBlocks / 2) : lean ? 2048 : 1024;
     }
     const int blocks = (int)std::min<int64_t>((rounds + a.inner - 1) / a.inner, most);
     a.jump = ((int64_t)blocks * a.inner - (a.inner - 1)) * rows;
