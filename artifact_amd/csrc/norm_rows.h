@@ -501,7 +501,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
     __shared__ typename ParamOf<Map, RELU>::Store bstore;
     float dw[K][V], db[K][V], wmost, bmost;
     const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, wmost);
-    const ParamOf<Map, RELU> bias(m, a.bias, 0.f, 1.f, bstore, bmost);   // pre = 1 in columns that do not exist: never near the border
+    // in columns that do not exist pre is -infinity: never near the border, and the gate is closed
+    const ParamOf<Map, RELU> bias(m, a.bias, 0.f, -__builtin_inff(), bstore, bmost);
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
@@ -530,7 +531,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
         dout.advance(go.step, all, further);
         next_x.template load<STREAM>(m, x.at);
         next_d.template load<STREAM>(m, dout.at);
-        // (columns that do not exist hold other columns of d: their weight is 0, and their sums are not stored)
+        // Columns that do not exist hold other columns of d.  Their weight is 0 and their sums are not stored, but an infinity
+        // or a NaN that the dropout or the gate stops in its own column has to be stopped there as well, so both do.
         if (go.left < Map::ROWS) {   // lane groups behind the last row work on it once more and add nothing
 #pragma unroll
             for (int j = 0; j < K; ++j)
@@ -550,7 +552,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
                 bool keep[V];
                 drop_kept(drop, group, (uint32_t)m.col(j), keep);
 #pragma unroll
-                for (int e = 0; e < V; ++e) d[j][e] = keep[e] ? d[j][e] : 0.f;
+                for (int e = 0; e < V; ++e) d[j][e] = keep[e] && (RELU || m.has(j, e)) ? d[j][e] : 0.f;
             }
         }
         if constexpr (RELU) {

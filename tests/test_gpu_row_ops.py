@@ -532,3 +532,24 @@ def test_modules_follow_their_mode():
     d = ROF_Dropout(0.5)
     assert torch.equal(d(x, rng, 2), dropout(x, 0.5, rng, 2))
     assert d.eval()(x, None) is x
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), -float("inf")])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("f", [2, 7, 47, 100, 300, 517, 1500, 4099, 6001])
+@pytest.mark.parametrize("relu,p", [(True, 0.0), (False, 0.5), (True, 0.5)])
+def test_a_gradient_that_is_masked_may_be_anything(f, dtype, bad, relu, p):
+    """Where the ReLU or the dropout stops the gradient, infinity and NaN in it leave dx and the parameters' gradients as
+    they were, in the last column too, whose vector also covers columns that the row does not have."""
+    n = 13
+    x, (w, b), dy = rows_of(n, f, dtype, 1), params(f, 2), rows_of(n, f, dtype, 3)
+    want = check_norm(x, w, b, dy, relu, p)
+    rows = np.arange(n)
+    keep = kept(rows, f, p, SEED, OFFSET) if p else np.ones((n, f), dtype=bool)
+    gone = ~keep | (relu & (Norm(host(x), host(w), host(b)).pre <= 0))
+    assert gone[:, -1].any() and gone[:, :-1].any()
+    dy[torch.from_numpy(gone).cuda()] = bad
+    x = x.detach().requires_grad_(True)
+    y = layer_norm(x, w, b, relu=relu, dropout=p, rng=rng_tensor())
+    for got, t in zip(torch.autograd.grad(y, (x, w, b), dy), want[1:]):
+        assert torch.equal(got, t)
