@@ -59,16 +59,21 @@ bool rows_apart(const Tensor &t) {
 }
 void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+void check_tangent(const char *name, const Tensor &t) {
+    require(!t._fw_grad(0).defined(), name, " must not carry a forward-mode tangent (there is no forward-mode derivative)");
+}
 void check_rows(const char *name, const Tensor &t) {
     require(t.is_cuda() && t.dim() == 2 && known(t.scalar_type()), name, " must be a 2-D float32 or bfloat16 CUDA tensor");
     require(t.size(1) > 0 && t.size(1) <= INT32_MAX, name, " must have at least one column");
     require(rows_apart(t), name, " must have unit column stride and rows that do not overlap");
-    require(!t._fw_grad(0).defined(), name, " must not carry a forward-mode tangent (there is no forward-mode derivative)");
+    require(!t.is_neg(), name, " must not be a view with the negative bit (resolve it first)");
+    check_tangent(name, t);
 }
 void check_param(const char *name, const Tensor &t, const Tensor &x) {
     require(!t.defined() || (t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 1 &&
-                             t.numel() == x.size(1) && t.is_contiguous()),
+                             t.numel() == x.size(1) && t.is_contiguous() && !t.is_neg()),
             name, " must be a contiguous float32 vector with one element per column on the device of x");
+    if (t.defined()) check_tangent(name, t);
 }
 void check_rate(double p) { require(p >= 0.0 && p <= 1.0, "a dropout rate must lie between 0 and 1"); }
 void check_rng(const Tensor &rng, const Tensor &x) {
@@ -79,6 +84,8 @@ void check_rng(const Tensor &rng, const Tensor &x) {
 
 // An incoming gradient as rows the kernels take: autograd hands over broadcast and transposed ones as well.
 Tensor gradient_rows(Tensor grad, at::ScalarType type) {
+    check_tangent("the gradient", grad);
+    grad = grad.resolve_neg();
     if (grad.scalar_type() != type) grad = grad.to(type);
     return rows_apart(grad) ? grad : grad.contiguous();
 }

@@ -553,3 +553,32 @@ def test_a_gradient_that_is_masked_may_be_anything(f, dtype, bad, relu, p):
     y = layer_norm(x, w, b, relu=relu, dropout=p, rng=rng_tensor())
     for got, t in zip(torch.autograd.grad(y, (x, w, b), dy), want[1:]):
         assert torch.equal(got, t)
+
+
+def test_views_and_derivatives_that_are_refused():
+    x, rng, w = torch.randn(6, 8, device="cuda"), rng_tensor(), torch.ones(8, device="cuda")
+    dual_level, make_dual = torch.autograd.forward_ad.dual_level, torch.autograd.forward_ad.make_dual
+    calls = [lambda t: layer_norm(t), lambda t: dropout(t, 0.5, rng)]
+    for call in calls:
+        with pytest.raises(RofError, match="negative"):
+            call(x._neg_view())
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(x)
+        with pytest.raises(RuntimeError):
+            torch.vmap(call)(x[None])
+        with dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            t = x.detach().requires_grad_(True)
+            torch.autograd.grad(call(t), t, make_dual(x, x))
+    with pytest.raises(RofError, match="weight"):
+        layer_norm(x, w._neg_view())
+    with dual_level():
+        with pytest.raises(RofError, match="forward-mode"):
+            layer_norm(x, make_dual(w, w))
+        with pytest.raises(RofError, match="forward-mode"):
+            layer_norm(x, w, make_dual(w, w))
+
+
+def test_a_gradient_with_the_negative_bit():
+    x, dy = rows_of(6, 8, "float32", 1).requires_grad_(True), rows_of(6, 8, "float32", 2)
+    for call in (lambda: layer_norm(x), lambda: dropout(x, 0.5, rng_tensor())):
+        assert torch.equal(torch.autograd.grad(call(), x, dy._neg_view())[0], torch.autograd.grad(call(), x, -dy)[0])
