@@ -311,14 +311,14 @@ struct Scratch {
     double part64[2][WAVES][2];
 };
 
-// A lane's columns of a parameter.  In registers where a row is part of a wavefront or a wavefront; in LDS where it is
-// several, because there a lane holds up to 32 columns, and it is registers (of the gradient's sums above all) that
-// bound the wavefronts in flight: 20011 rows of 4099 bfloat16 columns take the backward launch 180 us with them in registers,
-// 128 from LDS.  A lane reads back only what it wrote, 16 bytes at a time in lane order, so there is neither a barrier nor
-// a conflict.
-template <typename Map>
+// A lane's columns of a parameter.  In registers, but in LDS in the backward kernel of rows that are several wavefronts:
+// there a lane holds up to 32 columns, and it is registers (of the gradient's sums above all) that bound the wavefronts in
+// flight (20011 x 4099 bfloat16 with ReLU and dropout: 226 us with them in registers, 158 from LDS; without ReLU 113 either
+// way, and the forward kernel, which has registers to spare, 2 to 10 % slower from LDS).  A lane reads back only what it
+// wrote, 16 bytes at a time in lane order, so there is neither a barrier nor a conflict.
+template <typename Map, bool BACKWARD>
 struct Param {
-    static constexpr bool kLds = Map::WAVES_ > 1;
+    static constexpr bool kLds = BACKWARD && Map::WAVES_ > 1;
     static constexpr int V = Map::V, K = Map::K_, Q = V / 4;
     using Store = float4[kLds ? K * Q * Map::LANES : 1];
     float v[kLds ? 1 : K][V];
@@ -362,6 +362,10 @@ struct Param {
     }
 };
 
+// Forward.  A lane group works on one row while its next one is on its way; reads and writes the matrix once.  Alone on the
+// card, of the bytes it moves: 2^18 x 256 float32 99 us, 5.4 TB/s; 2.4 M x 47 float32 185 us, 4.9; 20011 x 4099 bfloat16 71 us,
+// 4.6; with ReLU and dropout 10^6 x 100 float32 151 us, 5.3; 2^22 x 256 bfloat16 820 us, 5.2 (a copy reaches 4.5 to 5.9);
+// 16384 x 16 float32 3 us, which is a launch.
 template <typename TX, typename TY, int LPR, int WAVES, int K>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd_kernel(NormArgs a) {
     using Map = RowMap<TX, LPR, WAVES, K>;
@@ -369,10 +373,10 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
     __shared__ Scratch<WAVES> sh;
     const Map m(a.f);
     int turn = 0;
-    __shared__ typename Param<Map>::Store wstore, bstore;
+    __shared__ typename Param<Map, false>::Store wstore, bstore;
     float most;
     // the dropout's scale is in the parameters: it is positive, so it passes through the ReLU
-    const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, most, a.scale), bias(m, a.bias, 0.f, 0.f, bstore, most, a.scale);
+    const Param<Map, false> weight(m, a.weight, 1.f, 0.f, wstore, most, a.scale), bias(m, a.bias, 0.f, 0.f, bstore, most, a.scale);
     const float f = (float)a.f, inv_f = 1.0f / f, eps = (float)a.eps;
     const int64_t first = Rounds::first<Map::ROWS>(a);
     Rounds go(a, first, Map::ROWS);
@@ -488,8 +492,13 @@ struct NoParam {
     __device__ __forceinline__ NoParam(const Map &, const float *, float, float, Store &, float &) {}
 };
 template <typename Map, bool NEEDED>
-using ParamOf = std::conditional_t<NEEDED, Param<Map>, NoParam>;
+using ParamOf = std::conditional_t<NEEDED, Param<Map, true>, NoParam>;
 
+// Backward.  As forward, with the gradient's row beside that of x: two reads and a write, and the parameters' gradients of the
+// workgroup's rows in registers up to its end.  Measured alike: 2.4 M x 47 float32 267 us, 5.1 TB/s; 2^20 x 64 bfloat16 64 us, 6.3
+// (a third of it from the Infinity Cache); 20011 x 4099 bfloat16 120 us, 4.1 (six vectors in flight per lane are what its registers hold);
+// with ReLU and dropout 10^6 x 100 float32 223 us, 5.4; 2^22 x 256 bfloat16 1215 us, 5.3; 16384 x 16 float32 4.5 us.
+// Two rows ahead instead of one are no gain (2^22 x 256 bfloat16 1425 us, with one 1355, before the launch was cut into tiles).
 template <typename TX, typename TY, int LPR, int WAVES, int K, bool RELU, bool STREAM>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd_kernel(NormArgs a) {
     using Map = RowMap<TX, LPR, WAVES, K>;
@@ -497,10 +506,10 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
     __shared__ Scratch<WAVES> sh;
     const Map m(a.f);
     int turn = 0, turn64 = 0;
-    __shared__ typename Param<Map>::Store wstore;
+    __shared__ typename Param<Map, true>::Store wstore;
     __shared__ typename ParamOf<Map, RELU>::Store bstore;
     float dw[K][V], db[K][V], wmost, bmost;
-    const Param<Map> weight(m, a.weight, 1.f, 0.f, wstore, wmost);
+    const Param<Map, true> weight(m, a.weight, 1.f, 0.f, wstore, wmost);
     // in columns that do not exist pre is -infinity: never near the border, and the gate is closed
     const ParamOf<Map, RELU> bias(m, a.bias, 0.f, -__builtin_inff(), bstore, bmost);
 #pragma unroll
