@@ -175,7 +175,7 @@ float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (
 // others twice per row, and as few idle lanes; bfloat16:
 //   385 000 x 520, 65 vectors, with ReLU and dropout: 32 lanes with three 153 / 271, 64 with two 186 / 356;
 //   39 000 x 2048, 256 vectors: two wavefronts with two vectors 57 / 83, one with four 54 / 93, four with one 56 / 83;
-//   20011 x 4099, 513 vectors: three with three 62 / 112, four with three 78 / 117, eight with two 89 / 159;
+//   20011 x 4099, 513 vectors: three with three 62 / 112, four with three 67 / 117, eight with two 89 / 159;
 //   9765 x 8192, 1024 vectors: eight with two 54 / 86, four with four 55 / 98.
 NormShape norm_shape(int f, int x_dtype) {
     // In every entry the vectors of a lane but its last are whole, because the entry before it ends at (k - 1) lpr waves or later.
