@@ -5,6 +5,7 @@ import ctypes as C
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from artifact_amd import _lib, row_ops
 from artifact_amd._lib import DropoutOpts, RofError
@@ -109,7 +110,8 @@ def test_more_rows_than_one_launch_holds_at_a_time(n, f, dtype):
     check_norm(rows_of(n, f, dtype, 5), w, b, rows_of(n, f, dtype, 6), True, 0.5)
 
 
-@pytest.mark.parametrize("dtype,n,f", [("float32", (1 << 18) + 3, 200), ("bfloat16", (1 << 18) + 77, 500), ("float32", (1 << 20) + 5, 33)])
+@pytest.mark.parametrize("dtype,n,f", [("float32", (1 << 18) + 3, 200), ("bfloat16", (1 << 18) + 77, 500), ("float32", (1 << 20) + 5, 33),
+                                       ("float32", (1 << 24) + 3, 3), ("bfloat16", (1 << 24) + 259, 5), ("float32", (1 << 23) + 1, 7)])
 def test_parameter_gradients_of_matrices_in_tiles(dtype, n, f):
     """So many rows that the backward launch leaves thousands of partial rows, which two more launches add up.  The 64-bit
     form is evaluated on the GPU here; the tolerances are row_oracle's."""
@@ -582,3 +584,35 @@ def test_a_gradient_with_the_negative_bit():
     x, dy = rows_of(6, 8, "float32", 1).requires_grad_(True), rows_of(6, 8, "float32", 2)
     for call in (lambda: layer_norm(x), lambda: dropout(x, 0.5, rng_tensor())):
         assert torch.equal(torch.autograd.grad(call(), x, dy._neg_view())[0], torch.autograd.grad(call(), x, -dy)[0])
+
+
+def test_what_the_backward_pass_keeps_is_watched_over():
+    dy = rows_of(6, 8, "float32", 2)
+    for which in range(3):
+        x, (w, b) = rows_of(6, 8, "float32", 1).requires_grad_(True), params(8, 3)
+        y = layer_norm(x, w, b, relu=True)
+        with torch.no_grad():
+            (x, w, b)[which].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, (x, w, b), dy)
+    x, (w, b) = rows_of(6, 8, "float32", 1).requires_grad_(True), params(8, 3)
+    for call in (lambda: layer_norm(x, w, b, relu=True, dropout=0.5, rng=rng_tensor()), lambda: dropout(x, 0.5, rng_tensor())):
+        y = call()
+        want = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+        with pytest.raises(RuntimeError, match="a second time"):
+            torch.autograd.grad(y, x, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = call()
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+
+
+def test_a_checkpointed_part_draws_the_mask_of_its_first_pass():
+    state, dy = ROF_DropoutState(3).cuda(), rows_of(40, 16, "float32", 2)
+    x, (w, b) = rows_of(40, 16, "float32", 1).requires_grad_(True), params(16, 3)
+    part = lambda x, rng: dropout(layer_norm(x, w, b, relu=True, dropout=0.5, rng=rng), 0.3, rng, call=1) * 2   # noqa: E731
+    rng = state.next(2)
+    want = torch.autograd.grad(part(x, rng), (x, w, b), dy)
+    y = torch.utils.checkpoint.checkpoint(part, x, rng, use_reentrant=False)
+    state.next(2)
+    assert all(torch.equal(g, t) for g, t in zip(torch.autograd.grad(y, (x, w, b), dy), want))
