@@ -81,6 +81,15 @@ __device__ __forceinline__ double group_sum(double v) {
     return v;
 }
 
+// The sum of a lane's N numbers as a balanced tree: as many additions as in a row, but each number passes ceil(log2 N).
+template <int N>
+__device__ __forceinline__ float tree_sum(const float *v) {
+    if constexpr (N == 1)
+        return v[0];
+    else
+        return tree_sum<(N + 1) / 2>(v) + tree_sum<N / 2>(v + (N + 1) / 2);
+}
+
 // s / f from the reciprocal, with what the product leaves of s added: a row of equal numbers (a node without in-edges under
 // a constant bias) has exactly that number as its mean, and no spread, where r = 1 / sqrt(eps) would magnify one rounding.
 __device__ __forceinline__ float mean_of(float s, float f, float inv_f) {
@@ -219,26 +228,26 @@ struct RowMap {
 
     // Mean of a row's elements and the sum of the squares of their differences from it; v becomes the differences (0 where
     // there is no column).  Of several wavefronts each takes its own columns' first, and the row's follow from theirs: the
-    // squares are theirs plus (columns) (their mean - the mean)^2, one barrier for both.
+    // squares are theirs plus (columns) (their mean - the mean)^2, one barrier for both.  `apart`: how far the mean of the
+    // wavefront's columns is from the row's.
     __device__ __forceinline__ void moments(float (&v)[K][V], float f, float inv_f, float (*part)[WAVES][2], int &turn, float &mean,
-                                            float &squares) const {
-        float s = 0.f;
+                                            float &squares, float &apart) const {
         if (!full) {
 #pragma unroll
             for (int e = 0; e < V; ++e) v[K - 1][e] = has(K - 1, e) ? v[K - 1][e] : 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += v[j][e];
-        s = group_sum<LPR>(s);
-        float own = WAVES > 1 ? mean_of(s, columns, inv_columns) : mean_of(s, f, inv_f), q = 0.f;   // columns: the wavefront's
+        float s = group_sum<LPR>(tree_sum<K * V>(&v[0][0]));
+        float own = WAVES > 1 ? mean_of(s, columns, inv_columns) : mean_of(s, f, inv_f);   // columns: the wavefront's
         subtract(v, own);
+        constexpr int CHAINS = K * V < 8 ? 2 : 4;   // of K V / CHAINS products each
+        float c[CHAINS];
 #pragma unroll
-        for (int j = 0; j < K; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) q = fmaf(v[j][e], v[j][e], q);
-        q = group_sum<LPR>(q);
+        for (int i = 0; i < K * V; ++i) {
+            const float d = v[i / V][i % V];
+            c[i % CHAINS] = i < CHAINS ? d * d : fmaf(d, d, c[i % CHAINS]);
+        }
+        float q = group_sum<LPR>(tree_sum<CHAINS>(c));
+        apart = 0.f;
         if constexpr (WAVES > 1) {
             float(*p)[2] = part[turn];
             turn ^= 1;
@@ -257,6 +266,7 @@ struct RowMap {
                 const float d = p[i][0] - own;
                 q += fmaf(columns_of((int)f, i) * d, d, p[i][1]);
             }
+            apart = fabsf(own - first);
             subtract(v, own - first);
         }
         mean = own;
@@ -313,7 +323,7 @@ struct Scratch {
 
 // A lane's columns of a parameter.  In registers, but in LDS in the backward kernel of rows that are several wavefronts:
 // there a lane holds up to 32 columns, and it is registers (of the gradient's sums above all) that bound the wavefronts in
-// flight (20011 x 4099 bfloat16 with ReLU and dropout: 226 us with them in registers, 158 from LDS; without ReLU 113 either
+// flight (20011 x 4099 bfloat16 with ReLU and dropout: 210 us with them in registers, 141 from LDS; without ReLU 113 either
 // way, and the forward kernel, which has registers to spare, 2 to 10 % slower from LDS).  A lane reads back only what it
 // wrote, 16 bytes at a time in lane order, so there is neither a barrier nor a conflict.
 template <typename Map, bool BACKWARD>
@@ -394,8 +404,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
         next.unpack(m, v);
         x.advance(go.step, all, further);
         next.template load<false>(m, x.at);   // on its way while this row is worked on
-        float mean, squares;
-        m.moments(v, f, inv_f, sh.part, turn, mean, squares);
+        float mean, squares, apart;
+        m.moments(v, f, inv_f, sh.part, turn, mean, squares, apart);
         const float r = rsqrtf(fmaf(squares, inv_f, eps));
 #pragma unroll
         for (int j = 0; j < K; ++j) {
@@ -424,13 +434,24 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd
 // The ReLU's gate decides whether a whole gradient passes, so its border must not move with the order in which a variant
 // of this kernel adds.  Where |pre| is within the rounding error that 32 bits can have there, the wavefront (or the
 // workgroup that shares the row) takes the row's statistics again in 64 bits and decides by those.  The bound, in half
-// steps u = 2^-24: a lane adds up to 32 numbers, the butterfly 6 more, the wavefronts' means are rounded and weighted (3) and
-// up to 16 of them added, so m is off by q / r with q = 58 u (|m| r + 1); h by q + 36 u |h| + |h| q^2 / 2, and the last
-// operation adds 2 u (|h w| + |b|).  Near the border |h w| is |b|, and for |m| r up to 2^10 q^2 / 2 is below 100 u, so all
-// of it is below 128 u = 2^-17 times |w| (2 |m| r + 1) + 2 |b|; for w and b a lane's largest serve, so that the common path
-// has one minimum per element.  A row whose mean is further from zero is always decided in 64 bits.  About 4 elements in
-// 10^5 are that close on normally distributed rows.
-constexpr float kBorder = 7.62939453125e-06f;
+// steps u = 2^-24, with F = |m| r + 1, which mean|x| r is at most, for a row of one wavefront or less:
+//   m: 5 additions in a lane, 6 across, 2 for the division: 13 u of mean|x|, so h is off by q = 13 u F;
+//   the squares: 2 u from the differences, 8 in a lane, 6 across: 16 u, so r by 8 u, by 3 u from its own operations (the sum
+//   with eps, the root), and by q^2 / 2 from m, which is 6 u for |m| r up to kFarMean; h by 2 u more: 19 u |h|.  Near the
+//   border |h w| is |b|, and the last operation adds 2 u |b|: in all 13 u F |w| + 21 u |b|.
+// For several wavefronts:
+//   m: 10 u more (eight weighted means, 2 for the division): 23 u F;  the difference is taken in two steps, off by u of
+//   its wavefront's mean's distance from m (`apart`) twice, and by u |h| once more;
+//   the squares: 2 u more in a lane, 12 u for the wavefronts', so r by 15 + 3 + 17 u; and the error e of a wavefront's
+//   mean counts once with that mean's distance from m: 2 e (distance) (columns) summed over the wavefronts is at most
+//   2 * 13 u F of the squares (Cauchy and Schwarz), r by 13 u F: 38 u |h| + 13 u F |h|;  in all 23 u F |w| + 2 u r (apart) |w| +
+//   (40 + 13 F) u |b|.
+// So 32 u and 64 u times F (|w| + |b|) + r (apart) |w|; for w and b a lane's largest serve, so that the common path has
+// one minimum per element.  A row whose mean is further from zero than kFarMean / r is always decided in 64 bits.  About 4
+// elements in 10^6 are that close on normally distributed rows, 8 in rows of several wavefronts.  (20011 x 4099 bfloat16 with
+// ReLU and dropout: 141 us; 130 if none ever came here, 159 with a border of four times the width.)
+template <int WAVES>
+constexpr float kBorder = WAVES > 1 ? 3.814697265625e-06f : 1.9073486328125e-06f;
 constexpr float kFarMean = 1024.f;
 
 // The exact sign of pre, in place of its value.  Rare, so it is kept out of the registers of the common path: the row is read
@@ -497,7 +518,7 @@ using ParamOf = std::conditional_t<NEEDED, Param<Map, true>, NoParam>;
 // Backward.  As forward, with the gradient's row beside that of x: two reads and a write, and the parameters' gradients of the
 // workgroup's rows in registers up to its end.  Measured alike: 2.4 M x 47 float32 267 us, 5.1 TB/s; 2^20 x 64 bfloat16 64 us, 6.3
 // (a third of it from the Infinity Cache); 20011 x 4099 bfloat16 120 us, 4.1 (six vectors in flight per lane are what its registers hold);
-// with ReLU and dropout 10^6 x 100 float32 223 us, 5.4; 2^22 x 256 bfloat16 1215 us, 5.3; 16384 x 16 float32 4.5 us.
+// with ReLU and dropout 10^6 x 100 float32 223 us, 5.4; 2^22 x 256 bfloat16 1205 us, 5.3; 16384 x 16 float32 4.5 us.
 // Two rows ahead instead of one are no gain (2^22 x 256 bfloat16 1425 us, with one 1355, before the launch was cut into tiles).
 template <typename TX, typename TY, int LPR, int WAVES, int K, bool RELU, bool STREAM>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd_kernel(NormArgs a) {
@@ -548,8 +569,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
 #pragma unroll
                 for (int e = 0; e < V; ++e) d[j][e] = ok ? d[j][e] : 0.f;
         }
-        float mean, squares;
-        m.moments(h, f, inv_f, sh.part, turn, mean, squares);
+        float mean, squares, apart;
+        m.moments(h, f, inv_f, sh.part, turn, mean, squares, apart);
         const float r = rsqrtf(fmaf(squares, inv_f, eps));
 #pragma unroll
         for (int j = 0; j < K; ++j)
@@ -578,7 +599,7 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
                 }
             }
             const float far = r * fabsf(mean);
-            const bool close = ok && (far > kFarMean || least <= kBorder * fmaf(fmaf(2.f, far, 1.f), wmost, 2.f * bmost));
+            const bool close = ok && (far > kFarMean || least <= kBorder<WAVES> * fmaf(far + 1.f, wmost + bmost, r * apart * wmost));
             if (WAVES > 1 ? __syncthreads_or(close) : __any(close)) gate64(m, a, here, weight, bias, sh.part64, turn64, pre);
 #pragma unroll
             for (int j = 0; j < K; ++j)

@@ -165,15 +165,15 @@ float drop_scale(int threshold) { return threshold < 65536 ? (float)(65536.0 / (
 // that holds it: few registers, and the rows of a wavefront are one contiguous piece.  Measured (us, forward / backward, each
 // with the launch size that suits it best):
 //   2^20 x 64 bfloat16, 8 vectors: 8 lanes 40 / 70, 4 lanes with two vectors 39 / 75, 16 lanes half empty 50 / 96;
-//   2^22 x 256 bfloat16, 32 vectors, with ReLU and dropout: 32 lanes 742 / 1125, 16 with two 736 / 1194;
+//   2^22 x 256 bfloat16, 32 vectors, with ReLU and dropout: 32 lanes 738 / 1111, 16 with two 739 / 1141;
 //   2^18 x 256 float32, 64 vectors: 64 lanes 92 / 134, 32 lanes with two vectors 92 / 131.
 // A group of 16 or more lanes of which that would leave a quarter idle is half as many lanes with two vectors (float32) or a
 // quarter with three (bfloat16, whose arithmetic per byte is twice as much); with ReLU and dropout:
-//   667 000 x 150 float32, 38 vectors: 32 lanes with two 147 / 240, 64 lanes 173 / 277, 16 with three 147 / 242;
-//   667 000 x 300 bfloat16, 38 vectors: 16 lanes with three 153 / 261, 64 lanes 213 / 348, 32 with two 177 / 339.
+//   667 000 x 150 float32, 38 vectors: 32 lanes with two 147 / 234, 64 lanes 173 / 275, 16 with three 146 / 233;
+//   667 000 x 300 bfloat16, 38 vectors: 16 lanes with three 153 / 245, 64 lanes 209 / 348, 32 with two 180 / 322.
 // Above that two or three vectors per lane and as few wavefronts as that takes, because every wavefront more waits for the
 // others twice per row, and as few idle lanes; bfloat16:
-//   385 000 x 520, 65 vectors, with ReLU and dropout: 32 lanes with three 153 / 271, 64 with two 186 / 356;
+//   385 000 x 520, 65 vectors, with ReLU and dropout: 32 lanes with three 153 / 246, 64 with two 188 / 340;
 //   39 000 x 2048, 256 vectors: two wavefronts with two vectors 57 / 83, one with four 54 / 93, four with one 56 / 83;
 //   20011 x 4099, 513 vectors: three with three 62 / 112, four with three 67 / 117, eight with two 89 / 159;
 //   9765 x 8192, 1024 vectors: eight with two 54 / 86, four with four 55 / 98.

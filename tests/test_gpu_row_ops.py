@@ -616,3 +616,23 @@ def test_a_checkpointed_part_draws_the_mask_of_its_first_pass():
     y = torch.utils.checkpoint.checkpoint(part, x, rng, use_reentrant=False)
     state.next(2)
     assert all(torch.equal(g, t) for g, t in zip(torch.autograd.grad(y, (x, w, b), dy), want))
+
+
+@pytest.mark.parametrize("dtype,mean", [("float32", 0.0), ("float32", 20.0), ("float32", 500.0), ("bfloat16", 20.0)])
+@pytest.mark.parametrize("f", [5, 47, 150, 256, 700, 1500, 2700, 4099, 8000])
+def test_the_relus_gate_in_rows_of_levels(f, dtype, mean):
+    """As above, with rows whose parts have means of their own, on both sides of the row's and far from zero: the error of a
+    wavefront's mean then counts in the row's spread as well."""
+    n = 96
+    level = torch.where(torch.arange(f) * 3 // f % 2 == 1, -1.0, 1.0) + mean
+    x = rows_of(n, f, dtype, f, mean=0.0)
+    x.copy_(0.05 * x.float() + level.cuda())
+    w, _ = params(f, 2)
+    o = Norm(host(x), host(w))
+    at = np.arange(f) % n
+    b = torch.from_numpy(-(o.h * o.w)[at, np.arange(f)].astype(np.float32)).cuda().requires_grad_(True)
+    o = Norm(host(x), host(w), host(b), relu=True)
+    db, = torch.autograd.grad(layer_norm(x, w, b, relu=True), b, torch.ones_like(x))
+    sure = (np.abs(o.pre) > 1e-12 * (1 + mean)).all(0)         # beyond the rounding of 64 bits
+    assert sure.mean() > 0.9
+    assert np.array_equal(host(db)[sure], o.gate.sum(0)[sure])
