@@ -51,7 +51,7 @@ template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
     constexpr int V = 16 / (int)sizeof(T), U = kTileVecs / 256;
     const Drop d(a);
-    const uint32_t groups = (uint32_t)(a.f + 7) / 8;
+    const uint32_t groups = ((uint32_t)a.f + 7) / 8;
     const int tail = a.f % V;
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
         const int64_t row0 = a.parts > 1 ? tile / a.parts : tile * a.rows;

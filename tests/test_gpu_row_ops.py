@@ -10,7 +10,7 @@ import torch.utils.checkpoint
 from artifact_amd import _lib, row_ops
 from artifact_amd._lib import DropoutOpts, RofError
 from artifact_amd.row_ops import ROF_Dropout, ROF_DropoutState, ROF_LayerNorm, dropout, layer_norm
-from row_oracle import HALF_STEP, U, Norm, kept, scale
+from row_oracle import HALF_STEP, U, Norm, kept, philox, scale, threshold
 
 pytestmark = pytest.mark.gpu
 
@@ -636,3 +636,21 @@ def test_the_relus_gate_in_rows_of_levels(f, dtype, mean):
     sure = (np.abs(o.pre) > 1e-12 * (1 + mean)).all(0)         # beyond the rounding of 64 bits
     assert sure.mean() > 0.9
     assert np.array_equal(host(db)[sure], o.gate.sum(0)[sure])
+
+
+@pytest.mark.parametrize("n,f", [(1, (1 << 31) - 1), (1, (1 << 31) - 8), (3, (1 << 30) + 5)])
+def test_dropout_of_the_longest_rows(n, f):
+    x = torch.full((n, f), 3.0, dtype=torch.bfloat16, device="cuda")
+    y = dropout(x, 0.25, rng_tensor())
+    groups = (f + 7) // 8
+    for row in range(n):
+        for first in (0, groups // 2 - 2, groups - 40):
+            g = np.arange(first, min(first + 40, groups))
+            i = g.astype(np.uint64) + np.uint64(row * groups)
+            c = np.zeros((len(i), 4), dtype=np.uint64)
+            c[:, 0], c[:, 1], c[:, 2], c[:, 3] = i & np.uint64(0xFFFFFFFF), i >> np.uint64(32), OFFSET & 0xFFFFFFFF, OFFSET >> 32
+            w = philox(c, (SEED & 0xFFFFFFFF, SEED >> 32))
+            u = np.stack([w & np.uint64(0xFFFF), w >> np.uint64(16)], -1).reshape(-1)
+            got = host(y[row, 8 * first: 8 * first + len(u)])
+            want = np.where(u >= threshold(0.25), host(torch.tensor(3 * scale(0.25), dtype=torch.float32).bfloat16()), 0.0)
+            assert np.array_equal(got, want[:len(got)]) and len(got) >= len(u) - 7
