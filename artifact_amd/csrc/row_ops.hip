@@ -283,7 +283,8 @@ int norm_args(NormArgs &a, const void *x, int x_dtype, int64_t ldx, int64_t n, i
 extern "C" {
 
 int rof_dropout_state_next(int64_t *state, int64_t calls, int64_t *used, void *stream) {
-    if (!state || !used || state == used || calls < 0 || !aligned(state, 8) || !aligned(used, 8)) return ROF_ERR_ARG;
+    if (!state || !used || calls < 0 || !aligned(state, 8) || !aligned(used, 8)) return ROF_ERR_ARG;
+    if ((uintptr_t)used < (uintptr_t)state + 16 && (uintptr_t)state < (uintptr_t)used + 16) return ROF_ERR_ARG;   // overlapping
     hipLaunchKernelGGL(dropout_state_next_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, state, calls, used);
     HIP_TRY(hipGetLastError());
     return ROF_OK;

@@ -121,7 +121,7 @@ def test_dropout_refuses_what_it_cannot_run(args, code):
 
 
 @pytest.mark.parametrize("state,calls,used", [(None, 1, PTR), (PTR, 1, None), (PTR, -1, PTR + 16), (PTR, 1, PTR),
-                                              (PTR + 4, 1, PTR + 16), (PTR, 1, PTR + 4)])
+                                              (PTR + 4, 1, PTR + 16), (PTR, 1, PTR + 4), (PTR, 1, PTR + 8), (PTR + 8, 1, PTR)])
 def test_dropout_state_refuses_what_it_cannot_run(state, calls, used):
     assert _lib.lib().rof_dropout_state_next(state, calls, used, None) == ARG
 
