@@ -332,8 +332,8 @@ int rof_dropout_state_next(int64_t *state, int64_t calls, int64_t *used, void *s
 /* Layer norm of every row, with the rest of a hidden layer in the same pass:
  *     out = dropout(relu(h * weight + bias)),   h = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)
  * weight, bias: device float32[f], or NULL for 1 and 0.  relu = 0 and dropout = NULL leave those out.  `out` is rounded
- * once.  Statistics are float32 over the row as read: h is off by up to 58 half steps (2^-24) of 1 + |mean| / spread, and
- * differences from the mean beyond 10^18 overflow their squares.  eps = 0 is taken at its word: a row without spread
+ * once.  Statistics are float32 over the row as read: h is off by up to 64 half steps (2^-24) of (1 + |h|) times
+ * 1 + |mean| / spread, and differences from the mean beyond 10^17 may overflow the sum of their squares.  eps = 0 is taken at its word: a row without spread
  * then becomes NaN.  A row is kept in one workgroup's registers, which limits it to ROF_LAYER_NORM_MAX_ROW_BYTES of
  * x (ROF_ERR_UNSUPPORTED otherwise). */
 #define ROF_LAYER_NORM_MAX_ROW_BYTES 32768
