@@ -13,10 +13,10 @@ namespace {
 
 using namespace rofn;
 
-// Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.  Where there
-// are more rounds of work than kManyRounds it is tiles of eight rounds, see norm_blocks, else workgroups that stay.
-constexpr int kBackwardBlocks = 1024, kBackwardTiles = 16384;
-constexpr int64_t kManyRounds = 65536;
+// Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.  From
+// kManyRounds rounds of work on it is tiles of four rounds, see norm_blocks, else workgroups that stay.
+constexpr int kBackwardBlocks = 1280, kBackwardTiles = 16384;
+constexpr int64_t kSomeRounds = 65536, kManyRounds = 100000;
 constexpr int kTiledColumns = 512;   // rows of more columns are several vectors per lane of a whole wavefront in either type
 constexpr int kParamsChunks = 128;   // rows that the first of two passes leaves of so many partial ones
 // An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
@@ -199,24 +199,31 @@ NormShape norm_shape(int f, int x_dtype) {
 // Forward: a workgroup per four adjacent rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
 // with 2048 workgroups that stay and step through the matrix together; 10^6 x 100 float32 142 / 155), else as many as stay:
 // 2048, or half as many where the lanes hold several vectors.
-// Backward: each workgroup leaves a row of partial sums.  With many rounds it is up to 16384 tiles of eight adjacent ones,
-// handed out as others end (2^22 x 256 bfloat16: 1221 us against 1355 with 1024 workgroups that stay, 2.4 M x 47 float32
-// 258 / 285, 10^6 x 100 233 / 272); with fewer 1024 that stay (2^20 x 64 bfloat16: 66 / 73), half as many where the lanes
-// hold several vectors, whose registers leave room for no more, and two adjacent rounds at a time (20011 x 4099 bfloat16
-// with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
-int norm_blocks(NormArgs &a, const NormShape &s, bool backward) {
+// Backward: each workgroup leaves a row of partial sums.  With many rounds it is tiles of four adjacent ones, handed out as
+// others end: up to 16384 for float32 (10^6 x 200 424 us; 4096 tiles 471, 1280 workgroups that stay 478; 2.4 M x 100 512 / 564 /
+// 570), up to 4096 for bfloat16, whose workgroups are fewer on a CU (1.6 M x 300 602, 16384 tiles 653, 1024 that stay 602; 2.4 M x
+// 47 171 / 184 / 170; 2^22 x 256 1132 / 1119 / 1207), and more launches and traffic for their sums.  With fewer rounds as many
+// workgroups stay as fit: five on a CU where a lane holds one float32 vector (2^18 x 256 to bfloat16 122 us, with four 127;
+// 10^5 rounds are where 5 us more for the sums pay), else four, or two where the lanes hold several vectors, whose registers leave
+// room for no more; four rounds at a time (131072 rounds: 269 us, one at a time 283), but one where there are few (37500 rounds
+// with 1024 workgroups: 77 us, with 1280 82) and two in wide rows (20011 x 4099 bfloat16 with four wavefronts: 106 us against
+// 117 one at a time; forward with three 62 / 71).
+int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
     const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
-    const bool lean = s.waves * s.lpr * s.k <= 64;   // rows of up to 64 vectors: kTiledColumns
+    const bool lean = s.waves * s.lpr * s.k <= 64, f32 = x_dtype == ROF_F32;   // lean: up to 64 vectors, see kTiledColumns
     int64_t most;
     if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
         a.inner = 4;
         most = kMostBlocks;
-    } else if (backward && lean && rounds >= kManyRounds) {
-        a.inner = 8;
-        most = kBackwardTiles;
-    } else {
+    } else if (!backward) {
         a.inner = lean || rounds < 2048 ? 1 : 2;
-        most = backward ? (lean || s.waves == 2 || s.lpr < 64 ? kBackwardBlocks : kBackwardBlocks / 2) : lean ? 2048 : 1024;
+        most = lean ? 2048 : 1024;
+    } else if (lean) {
+        a.inner = rounds >= kSomeRounds ? 4 : 1;
+        most = rounds >= kManyRounds ? (f32 ? kBackwardTiles : kBackwardTiles / 4) : rounds >= kSomeRounds && f32 && s.k == 1 ? 1280 : 1024;
+    } else {
+        a.inner = rounds < 2048 ? 1 : 2;
+        most = s.waves == 2 || s.lpr < 64 ? 1024 : 512;
     }
     const int blocks = (int)std::min<int64_t>((rounds + a.inner - 1) / a.inner, most);
     a.jump = ((int64_t)blocks * a.inner - (a.inner - 1)) * rows;
@@ -235,7 +242,7 @@ bool norm_streams(const NormArgs &a, const NormShape &s, int x_dtype, int y_dtyp
 
 int launch_norm(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st) {
     const NormShape s = norm_shape(a.f, x_dtype);
-    const int blocks = norm_blocks(a, s, false);
+    const int blocks = norm_blocks(a, s, x_dtype, false);
     if (x_dtype == ROF_F32) return y_dtype == ROF_F32 ? norm_fwd_f32_f32(a, s, blocks, st) : norm_fwd_f32_bf16(a, s, blocks, st);
     return y_dtype == ROF_F32 ? norm_fwd_bf16_f32(a, s, blocks, st) : norm_fwd_bf16_bf16(a, s, blocks, st);
 }
@@ -243,7 +250,7 @@ int launch_norm(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st) {
 int launch_norm_backward(NormArgs &a, int x_dtype, int y_dtype, hipStream_t st, int *blocks) {
     NormShape s = norm_shape(a.f, x_dtype);
     s.stream = norm_streams(a, s, x_dtype, y_dtype);
-    const int b = *blocks = norm_blocks(a, s, true);
+    const int b = *blocks = norm_blocks(a, s, x_dtype, true);
     if (x_dtype == ROF_F32) {
         if (y_dtype == ROF_F32) return a.relu ? norm_bwd_relu_f32_f32(a, s, b, st) : norm_bwd_f32_f32(a, s, b, st);
         return a.relu ? norm_bwd_relu_f32_bf16(a, s, b, st) : norm_bwd_f32_bf16(a, s, b, st);

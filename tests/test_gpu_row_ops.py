@@ -111,7 +111,10 @@ def test_more_rows_than_one_launch_holds_at_a_time(n, f, dtype):
 
 
 @pytest.mark.parametrize("dtype,n,f", [("float32", (1 << 18) + 3, 200), ("bfloat16", (1 << 18) + 77, 500), ("float32", (1 << 20) + 5, 33),
-                                       ("float32", (1 << 24) + 3, 3), ("bfloat16", (1 << 24) + 259, 5), ("float32", (1 << 23) + 1, 7)])
+                                       ("float32", (1 << 24) + 3, 3), ("bfloat16", (1 << 24) + 259, 5), ("float32", (1 << 23) + 1, 7),
+                                       ("float32", 400001, 200), ("float32", 399996, 256), ("float32", 399997, 200), ("bfloat16", 400033, 500),
+                                       ("float32", 3200001, 47), ("bfloat16", 1600019, 300), ("float32", 800005, 150),
+                                       ("float32", 25600003, 3), ("bfloat16", 12800077, 13)])
 def test_parameter_gradients_of_matrices_in_tiles(dtype, n, f):
     """So many rows that the backward launch leaves thousands of partial rows, which two more launches add up.  The 64-bit
     form is evaluated on the GPU here; the tolerances are row_oracle's."""

@@ -104,9 +104,9 @@ def test_backward_workspace_holds_a_row_per_workgroup():
     size = _lib.lib().rof_layer_norm_backward_workspace_bytes
     assert size(0, 8) == 0 and size(5, 0) == 0
     assert size(3, 8) == 3 * 2 * 8 * 4
-    assert size(65535, 47) == 1024 * 2 * 47 * 4
+    assert size(1280, 47) == size(99999, 47) == 1280 * 2 * 47 * 4
     assert size(10 ** 7, 47) == (16384 + 128) * 2 * 47 * 4 and size(10 ** 7, 512) == (16384 + 128) * 2 * 512 * 4
-    assert size(10 ** 7, 513) == 1024 * 2 * 513 * 4
+    assert size(10 ** 7, 513) == 1280 * 2 * 513 * 4
 
 
 @pytest.mark.parametrize("args,code", [
