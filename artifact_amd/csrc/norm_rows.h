@@ -516,9 +516,9 @@ template <typename Map, bool NEEDED>
 using ParamOf = std::conditional_t<NEEDED, Param<Map, true>, NoParam>;
 
 // Backward.  As forward, with the gradient's row beside that of x: two reads and a write, and the parameters' gradients of the
-// workgroup's rows in registers up to its end.  Measured alike: 2.4 M x 47 float32 267 us, 5.1 TB/s; 2^20 x 64 bfloat16 64 us, 6.3
-// (a third of it from the Infinity Cache); 20011 x 4099 bfloat16 120 us, 4.1 (six vectors in flight per lane are what its registers hold);
-// with ReLU and dropout 10^6 x 100 float32 223 us, 5.4; 2^22 x 256 bfloat16 1205 us, 5.3; 16384 x 16 float32 4.5 us.
+// workgroup's rows in registers up to its end.  Measured alike: 2.4 M x 47 float32 264 us, 5.1 TB/s; 2^20 x 64 bfloat16 64 us, 6.3
+// (a third of it from the Infinity Cache); 20011 x 4099 bfloat16 119 us, 4.1 (six vectors in flight per lane are what its registers hold);
+// with ReLU and dropout 10^6 x 100 float32 207 us, 5.8; 2^22 x 256 bfloat16 1228 us, 5.2; 16384 x 16 float32 4.5 us.
 // Two rows ahead instead of one are no gain (2^22 x 256 bfloat16 1425 us, with one 1355, before the launch was cut into tiles).
 template <typename TX, typename TY, int LPR, int WAVES, int K, bool RELU, bool STREAM>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd_kernel(NormArgs a) {

@@ -133,8 +133,8 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restri
     }
 }
 
-// Thousands of partial rows are first added up in kParamsChunks chunks, 64 columns of a chunk per workgroup (16384 rows of
-// 512 floats: 7 us, and 5 us for the other kernel behind it; that one alone would have them in 32 workgroups).
+// Thousands of partial rows are first added up in kParamsChunks chunks, 64 columns of a chunk per workgroup (4096 rows of
+// 512 floats: 5 us, and 5 us for the other kernel behind it; that one alone would have them in 32 workgroups).
 __global__ __launch_bounds__(256) void norm_params_chunk_kernel(const float *__restrict__ partial, int blocks, int f,
                                                                  float *__restrict__ out) {
     __shared__ float red[4][64];
