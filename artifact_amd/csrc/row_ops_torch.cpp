@@ -5,8 +5,14 @@
 //
 // Nothing but the inputs is kept for the backward pass.  Checks raise the exception type that set_error_type was given.
 //
+// They are registered with PyTorch's dispatcher (rof::layer_norm, rof::layer_norm_backward, rof::dropout,
+// rof::dropout_state_next), and every call goes through it, the backward pass's too.  What records a program from the calls
+// it sees (torch.jit.trace, make_fx) then sees these; without them it would see no more than the allocation of the
+// result, and replay that.  A replay calls the operators with other tensors, so the checks are theirs.
+//
 // Built by artifact_amd/build.py into artifact_amd/_ROFrows*.so.
 #include <torch/extension.h>
+#include <torch/library.h>
 
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -103,33 +109,136 @@ variable_list once(variable_list grads, const char *what) {
     return grads;
 }
 
-struct DropoutArgs {
-    double p = 0.0;
-    int64_t call = 0;
-};
+using LayerNorm = Tensor(const Tensor &, const std::optional<Tensor> &, const std::optional<Tensor> &, double, bool, double,
+                         const std::optional<Tensor> &, int64_t, std::optional<at::ScalarType>);
+using LayerNormBackward = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const std::optional<Tensor> &,
+                                                             const std::optional<Tensor> &, double, bool, double,
+                                                             const std::optional<Tensor> &, int64_t, at::ScalarType, bool, bool,
+                                                             bool);
+using Dropout = Tensor(const Tensor &, double, const std::optional<Tensor> &, int64_t);
+using DropoutStateNext = Tensor(const Tensor &, int64_t);
 
-Tensor run_dropout(const Tensor &x, const DropoutArgs &d, const Tensor &rng) {
+template <typename F>
+c10::TypedOperatorHandle<F> find(const char *name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+const auto &layer_norm_op() {
+    static const auto op = find<LayerNorm>("rof::layer_norm");
+    return op;
+}
+const auto &layer_norm_backward_op() {
+    static const auto op = find<LayerNormBackward>("rof::layer_norm_backward");
+    return op;
+}
+const auto &dropout_op() {
+    static const auto op = find<Dropout>("rof::dropout");
+    return op;
+}
+const auto &dropout_state_next_op() {
+    static const auto op = find<DropoutStateNext>("rof::dropout_state_next");
+    return op;
+}
+
+std::optional<Tensor> maybe(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// What the checks of the kernels below would not be reached with, or too late to be told plainly.
+void check_call(const Tensor &x) {
+    require(x.is_cuda() && x.layout() == at::kStrided, "x must be a 2-D float32 or bfloat16 CUDA tensor");
+}
+void check_plain(const std::optional<Tensor> &t) {
+    const c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
+    require(!t || !t->key_set().has_any(wrapped), "the row operators do not take part in torch.func's transforms");
+}
+
+// ---- on the device ------------------------------------------------------------------------------------------------
+Tensor dropout_cuda(const Tensor &x, double p, const std::optional<Tensor> &rng_, int64_t call) {
+    const Tensor rng = rng_.value_or(Tensor());
+    check_rows("x", x);
+    check_rate(p);
+    check_rng(rng, x);
     const c10::DeviceGuard guard(x.device());
     Tensor out = at::empty({x.size(0), x.size(1)}, x.options());
-    const rof_dropout_opts opts = {d.p, (const int64_t *)rng.data_ptr(), d.call};
+    const rof_dropout_opts opts = {p, (const int64_t *)rng.data_ptr(), call};
     check(rof_dropout(x.data_ptr(), type_of(x.scalar_type()), row_stride(x), x.size(0), (int)x.size(1), out.data_ptr(), x.size(1),
                       &opts, current_stream(x)),
           "dropout");
     return out;
 }
 
+void check_norm(const Tensor &x, const Tensor &weight, const Tensor &bias, double eps, double p, const Tensor &rng,
+                at::ScalarType out_type) {
+    check_rows("x", x);
+    require(x.size(1) * (int64_t)x.element_size() <= ROF_LAYER_NORM_MAX_ROW_BYTES,
+            "layer_norm takes rows of at most 32768 bytes (8192 float32 or 16384 bfloat16 columns)");
+    static_assert(ROF_LAYER_NORM_MAX_ROW_BYTES == 32768, "the message above");
+    check_param("weight", weight, x);
+    check_param("bias", bias, x);
+    require(eps >= 0.0 && eps <= 1e30, "eps must not be negative, and finite");
+    check_rate(p);
+    if (p > 0) check_rng(rng, x);
+    require(known(out_type), "out_dtype must be float32 or bfloat16");
+}
+
+Tensor layer_norm_cuda(const Tensor &x, const std::optional<Tensor> &weight_, const std::optional<Tensor> &bias_, double eps,
+                       bool relu, double p, const std::optional<Tensor> &rng_, int64_t call,
+                       std::optional<at::ScalarType> out_type_) {
+    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor()), rng = rng_.value_or(Tensor());
+    const at::ScalarType out_type = out_type_.value_or(x.scalar_type());
+    check_norm(x, weight, bias, eps, p, rng, out_type);
+    const c10::DeviceGuard guard(x.device());
+    Tensor out = at::empty({x.size(0), x.size(1)}, x.options().dtype(out_type));
+    const rof_dropout_opts opts = {p, p > 0 ? (const int64_t *)rng.data_ptr() : nullptr, call};
+    check(rof_layer_norm(x.data_ptr(), type_of(x.scalar_type()), row_stride(x), x.size(0), (int)x.size(1),
+                         (const float *)address(weight), (const float *)address(bias), eps, relu, p > 0 ? &opts : nullptr,
+                         out.data_ptr(), type_of(out_type), x.size(1), current_stream(x)),
+          "layer norm");
+    return out;
+}
+
+// out_type: that of the forward pass's result, which the gradient is taken to
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_cuda(const Tensor &grad_, const Tensor &x, const std::optional<Tensor> &weight_,
+                                                            const std::optional<Tensor> &bias_, double eps, bool relu, double p,
+                                                            const std::optional<Tensor> &rng_, int64_t call,
+                                                            at::ScalarType out_type, bool want_x, bool want_weight, bool want_bias) {
+    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor()), rng = rng_.value_or(Tensor());
+    check_norm(x, weight, bias, eps, p, rng, out_type);
+    require(grad_.device() == x.device() && grad_.sizes() == x.sizes(), "the gradient must be of x's shape and on its device");
+    const c10::DeviceGuard guard(x.device());
+    const Tensor grad = gradient_rows(grad_, out_type);
+    const int64_t n = x.size(0), f = x.size(1);
+    const auto floats = x.options().dtype(at::kFloat);
+    Tensor dx, dw, db, workspace;
+    if (want_x) dx = at::empty({n, f}, x.options());
+    if (want_weight) dw = at::empty({f}, floats);
+    if (want_bias) db = at::empty({f}, floats);
+    const size_t bytes = want_weight || want_bias ? rof_layer_norm_backward_workspace_bytes(n, (int)f) : 0;
+    if (bytes) workspace = at::empty({(int64_t)(bytes / sizeof(float))}, floats);
+    const rof_dropout_opts opts = {p, p > 0 ? (const int64_t *)rng.data_ptr() : nullptr, call};
+    check(rof_layer_norm_backward(grad.data_ptr(), type_of(out_type), row_stride(grad), x.data_ptr(), type_of(x.scalar_type()),
+                                  row_stride(x), n, (int)f, (const float *)address(weight), (const float *)address(bias), eps, relu,
+                                  p > 0 ? &opts : nullptr, address(dx), f, (float *)address(dw), (float *)address(db),
+                                  address(workspace), bytes, current_stream(x)),
+          "layer norm's gradient");
+    return {dx, dw, db};
+}
+
+// ---- differentiation ----------------------------------------------------------------------------------------------
 struct RofDropoutBackward : public Node {
     SavedVariable rng;
-    DropoutArgs args;
+    double p;
+    int64_t call;
     at::ScalarType type;
 
     variable_list apply(variable_list &&grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(1);
+        const Tensor state = rng.unpack();   // outside the guards: a checkpointed part runs its forward pass again here
         Tensor dx;
         {
             at::NoGradGuard quiet;
-            dx = run_dropout(gradient_rows(grads[0], type), args, rng.unpack());
+            const Tensor rows = gradient_rows(grads[0], type);
+            const at::AutoDispatchBelowADInplaceOrView below;
+            dx = dropout_op().call(rows, p, state, call);
         }
         return once({dx}, "dropout");
     }
@@ -140,65 +249,45 @@ struct RofDropoutBackward : public Node {
     std::string name() const override { return "RofDropoutBackward"; }
 };
 
-Tensor dropout(const Tensor &x, double p, const std::optional<Tensor> &rng_, int64_t call) {
-    const Tensor rng = rng_.value_or(Tensor());
-    check_rows("x", x);
-    check_rate(p);
-    check_rng(rng, x);
-    const DropoutArgs args = {p, call};
-    at::Tensor out;
+Tensor dropout_autograd(const Tensor &x, double p, const std::optional<Tensor> &rng, int64_t call) {
+    Tensor out;
     {
-        at::NoGradGuard quiet;
-        out = run_dropout(x, args, rng);
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = dropout_op().call(x, p, rng, call);
     }
     if (at::GradMode::is_enabled() && x.requires_grad()) {
         auto node = std::shared_ptr<RofDropoutBackward>(new RofDropoutBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x));
-        node->rng = SavedVariable(rng, false);
-        node->args = args;
+        node->rng = SavedVariable(*rng, false);
+        node->p = p;
+        node->call = call;
         node->type = x.scalar_type();
         torch::autograd::set_history(out, node);
     }
     return out;
 }
 
-struct NormArgs {
-    double eps;
-    bool relu;
-    DropoutArgs drop;
-    at::ScalarType out_type;
-};
-
 struct RofLayerNormBackward : public Node {
     SavedVariable x_, weight_, bias_, rng_;
-    NormArgs args;
+    double eps, p;
+    bool relu;
+    int64_t call;
+    at::ScalarType out_type;
 
     variable_list apply(variable_list &&grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined()) return variable_list(3);
+        // outside the guards, as above
         const Tensor x = x_.unpack(), weight = weight_.unpack(), bias = bias_.unpack(), rng = rng_.unpack();
-        Tensor dx, dw, db;
+        std::tuple<Tensor, Tensor, Tensor> d;
         {
             at::NoGradGuard quiet;
-            const c10::DeviceGuard guard(x.device());
-            const Tensor grad = gradient_rows(grads[0], args.out_type);
-            const int64_t n = x.size(0), f = x.size(1);
-            const auto floats = x.options().dtype(at::kFloat);
-            if (task_should_compute_output(0)) dx = at::empty({n, f}, x.options());
-            if (task_should_compute_output(1)) dw = at::empty({f}, floats);
-            if (task_should_compute_output(2)) db = at::empty({f}, floats);
-            Tensor workspace;
-            const size_t bytes = dw.defined() || db.defined() ? rof_layer_norm_backward_workspace_bytes(n, (int)f) : 0;
-            if (bytes) workspace = at::empty({(int64_t)(bytes / sizeof(float))}, floats);
-            const rof_dropout_opts opts = {args.drop.p, (const int64_t *)address(rng), args.drop.call};
-            check(rof_layer_norm_backward(grad.data_ptr(), type_of(args.out_type), row_stride(grad), x.data_ptr(),
-                                          type_of(x.scalar_type()), row_stride(x), n, (int)f, (const float *)address(weight),
-                                          (const float *)address(bias), args.eps, args.relu, args.drop.p > 0 ? &opts : nullptr,
-                                          address(dx), f, (float *)address(dw), (float *)address(db), address(workspace), bytes,
-                                          current_stream(x)),
-                  "layer norm's gradient");
+            const at::AutoDispatchBelowADInplaceOrView below;
+            d = layer_norm_backward_op().call(grads[0], x, maybe(weight), maybe(bias), eps, relu, p, maybe(rng), call, out_type,
+                                              task_should_compute_output(0), task_should_compute_output(1),
+                                              task_should_compute_output(2));
         }
-        return once({dx, dw, db}, "layer_norm");
+        return once({std::get<0>(d), std::get<1>(d), std::get<2>(d)}, "layer_norm");
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -210,35 +299,15 @@ struct RofLayerNormBackward : public Node {
     std::string name() const override { return "RofLayerNormBackward"; }
 };
 
-Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight_, const std::optional<Tensor> &bias_, double eps, bool relu,
-                  double p, const std::optional<Tensor> &rng_, int64_t call, std::optional<at::ScalarType> out_type) {
-    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
-    check_rows("x", x);
-    require(x.size(1) * (int64_t)x.element_size() <= ROF_LAYER_NORM_MAX_ROW_BYTES,
-            "layer_norm takes rows of at most 32768 bytes (8192 float32 or 16384 bfloat16 columns)");
-    static_assert(ROF_LAYER_NORM_MAX_ROW_BYTES == 32768, "the message above");
-    check_param("weight", weight, x);
-    check_param("bias", bias, x);
-    require(eps >= 0.0 && eps <= 1e30, "eps must not be negative, and finite");
-    check_rate(p);
-    Tensor rng;
-    if (p > 0) {
-        rng = rng_.value_or(Tensor());
-        check_rng(rng, x);
-    }
-    const NormArgs args = {eps, relu, {p, call}, out_type.value_or(x.scalar_type())};
-    require(known(args.out_type), "out_dtype must be float32 or bfloat16");
+Tensor layer_norm_autograd(const Tensor &x, const std::optional<Tensor> &weight_, const std::optional<Tensor> &bias_, double eps,
+                           bool relu, double p, const std::optional<Tensor> &rng, int64_t call,
+                           std::optional<at::ScalarType> out_type) {
     Tensor out;
     {
-        at::NoGradGuard quiet;
-        const c10::DeviceGuard guard(x.device());
-        out = at::empty({x.size(0), x.size(1)}, x.options().dtype(args.out_type));
-        const rof_dropout_opts opts = {p, (const int64_t *)address(rng), call};
-        check(rof_layer_norm(x.data_ptr(), type_of(x.scalar_type()), row_stride(x), x.size(0), (int)x.size(1),
-                             (const float *)address(weight), (const float *)address(bias), eps, relu, p > 0 ? &opts : nullptr,
-                             out.data_ptr(), type_of(args.out_type), x.size(1), current_stream(x)),
-              "layer norm");
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = layer_norm_op().call(x, weight_, bias_, eps, relu, p, rng, call, out_type);
     }
+    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()))) {
         auto node = std::shared_ptr<RofLayerNormBackward>(new RofLayerNormBackward(), torch::autograd::deleteNode);
@@ -246,16 +315,19 @@ Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight_, const s
         node->x_ = SavedVariable(x, false);
         node->weight_ = SavedVariable(weight, false);
         node->bias_ = SavedVariable(bias, false);
-        node->rng_ = SavedVariable(rng, false);
-        node->args = args;
+        node->rng_ = SavedVariable(p > 0 ? rng.value_or(Tensor()) : Tensor(), false);
+        node->eps = eps;
+        node->p = p;
+        node->relu = relu;
+        node->call = call;
+        node->out_type = out_type.value_or(x.scalar_type());
         torch::autograd::set_history(out, node);
     }
     return out;
 }
 
 // The values of one step, and the state moved on behind it.
-Tensor dropout_state_next(const Tensor &state, int64_t calls) {
-    require(state.is_cuda(), "the dropout state must be on the GPU (move the module there)");
+Tensor dropout_state_next_cuda(const Tensor &state, int64_t calls) {
     require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous(),
             "the dropout state must be a contiguous int64 tensor {seed, offset}");
     require(calls >= 0, "calls must not be negative");
@@ -267,7 +339,52 @@ Tensor dropout_state_next(const Tensor &state, int64_t calls) {
     return used;
 }
 
+// ---- Python's calls -----------------------------------------------------------------------------------------------
+Tensor layer_norm(const Tensor &x, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps, bool relu,
+                  double p, const std::optional<Tensor> &rng, int64_t call, std::optional<at::ScalarType> out_type) {
+    check_call(x);
+    check_plain(x);
+    for (const auto *t : {&weight, &bias, &rng}) check_plain(*t);
+    return layer_norm_op().call(x, weight, bias, eps, relu, p, rng, call, out_type);
+}
+Tensor dropout(const Tensor &x, double p, const std::optional<Tensor> &rng, int64_t call) {
+    check_call(x);
+    check_plain(x);
+    check_plain(rng);
+    return dropout_op().call(x, p, rng, call);
+}
+Tensor dropout_state_next(const Tensor &state, int64_t calls) {
+    require(state.is_cuda(), "the dropout state must be on the GPU (move the module there)");
+    check_plain(state);
+    return dropout_state_next_op().call(state, calls);
+}
+
 }  // namespace
+
+TORCH_LIBRARY(rof, m) {
+    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, bool relu, float dropout, Tensor? rng, int call, "
+          "ScalarType? out_dtype) -> Tensor");
+    m.def("layer_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, float eps, bool relu, float dropout, "
+          "Tensor? rng, int call, ScalarType out_dtype, bool want_x, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)");
+    m.def("dropout(Tensor x, float p, Tensor? rng, int call) -> Tensor");
+    m.def("dropout_state_next(Tensor(a!) state, int calls) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(rof, CUDA, m) {
+    m.impl("layer_norm", &layer_norm_cuda);
+    m.impl("layer_norm_backward", &layer_norm_backward_cuda);
+    m.impl("dropout", &dropout_cuda);
+    m.impl("dropout_state_next", &dropout_state_next_cuda);
+}
+TORCH_LIBRARY_IMPL(rof, AutogradCUDA, m) {
+    m.impl("layer_norm", &layer_norm_autograd);
+    m.impl("dropout", &dropout_autograd);
+    m.impl("dropout_state_next", torch::CppFunction::makeFallthrough());   // whole numbers
+}
+// views with the negative bit reach the kernels' checks, which refuse them
+TORCH_LIBRARY_IMPL(rof, Negative, m) {
+    for (const char *name : {"layer_norm", "layer_norm_backward", "dropout", "dropout_state_next"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
+}
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::register_exception_translator([](std::exception_ptr p) {

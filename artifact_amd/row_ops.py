@@ -3,7 +3,10 @@ ReLU and the dropout of a hidden layer in the same pass, and dropout whose mask 
 
 Not upstream: its models put torch's dropout on the input of every layer but the first (ROF_evaluation/ROF_main.py:192-200)
 and do not normalise.  `layer_norm` and `dropout` are differentiable functions of 2-D tensors with one row per node,
-`ROF_LayerNorm`, `ROF_Dropout` and `ROF_DropoutState` the modules that `ROF_GCN` and `ROF_GIN` are built from.
+`ROF_LayerNorm`, `ROF_Dropout` and `ROF_DropoutState` the modules that `ROF_GCN` and `ROF_GIN` are built from.  They are
+operators of PyTorch's dispatcher (rof::layer_norm, rof::layer_norm_backward, rof::dropout, rof::dropout_state_next), so
+torch.jit.trace and make_fx record them as calls; a traced program that is loaded in another process needs
+`rof_module.row_operators()` called there first.  torch.func's transforms are refused.
 """
 from __future__ import annotations
 

@@ -1,0 +1,125 @@
+"""How the row operators are called on the GPU: recorded programs, other streams, wrapped tensors."""
+import io
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from artifact_amd._lib import RofError
+from artifact_amd.row_ops import ROF_DropoutState, ROF_LayerNorm, dropout, layer_norm
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(n, f, seed, dtype=torch.float32):
+    return torch.randn(n, f, generator=torch.Generator().manual_seed(seed)).to("cuda", dtype)
+
+
+def params(f, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return ((1 + 0.3 * torch.randn(f, generator=gen)).cuda().requires_grad_(True),
+            (0.3 * torch.randn(f, generator=gen)).cuda().requires_grad_(True))
+
+
+def rng_tensor(seed=5, offset=3):
+    return torch.tensor([seed, offset], device="cuda")
+
+
+def through_a_file(traced):
+    buf = io.BytesIO()
+    torch.jit.save(traced, buf)
+    return torch.jit.load(io.BytesIO(buf.getvalue()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_traced_function_computes_what_it_traced(dtype):
+    (w, b), rng = (t.detach() for t in params(24, 1)), rng_tensor()     # the tracer takes no leaves as constants
+    calls = [lambda x: layer_norm(x, w, b), lambda x: layer_norm(x, w, b, relu=True, out_dtype=torch.bfloat16),
+             lambda x: layer_norm(x, None, b, relu=True, dropout=0.5, rng=rng, call=2), lambda x: dropout(x, 0.25, rng, call=1),
+             lambda x: dropout(layer_norm(x), 0.5, rng) * 2]
+    with torch.no_grad():
+        for call in calls:
+            traced = torch.jit.trace(call, (rows(7, 24, 2, dtype),))
+            assert "rof::" in str(traced.graph)
+            for n in (7, 13, 1):
+                x = rows(n, 24, 10 + n, dtype)
+                assert torch.equal(traced(x), call(x)) and torch.equal(through_a_file(traced)(x), call(x))
+
+
+def test_a_traced_program_checks_what_it_is_given():
+    w, b = (t.detach() for t in params(24, 1))
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda x: layer_norm(x, w, b), (rows(7, 24, 2),))
+        for bad in (rows(7, 23, 3), rows(7, 24, 3).half(), rows(7, 24, 3).cpu(), rows(24, 7, 3).t()):
+            with pytest.raises(RuntimeError):
+                traced(bad)
+
+
+def test_a_traced_module_draws_new_masks():
+    class Tail(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = ROF_LayerNorm(24, relu=True, dropout=0.5)
+            self.state = ROF_DropoutState(3)
+
+        def forward(self, x):
+            return self.norm(x, self.state.next(2), call=1)
+
+    m, other = Tail().cuda(), Tail().cuda()
+    x = rows(40, 24, 2)
+    with torch.no_grad():
+        traced = torch.jit.trace(m, (x,), check_trace=False)     # a check would compare two masks
+        m.state.state.copy_(torch.tensor([3, 0]))
+        for _ in range(3):
+            assert torch.equal(traced(x), other(x))
+        assert m.state.state.tolist() == other.state.state.tolist() == [3, 6]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_recorded_step_computes_its_gradients(dtype):
+    rng = rng_tensor()
+
+    def step(x, w, b, dy):
+        y = layer_norm(x, w, b, relu=True, dropout=0.5, rng=rng)
+        z = dropout(y, 0.25, rng, call=1)
+        return (z.detach(),) + torch.autograd.grad(z, (x, w, b), dy)
+
+    def inputs(n, seed):
+        return (rows(n, 24, seed, dtype).requires_grad_(True), *params(24, seed + 1), rows(n, 24, seed + 2, dtype))
+
+    recorded = make_fx(step)(*inputs(7, 1))
+    targets = {str(node.target) for node in recorded.graph.nodes}
+    assert {"rof.layer_norm.default", "rof.layer_norm_backward.default", "rof.dropout.default"} <= targets
+    for seed in (20, 30):
+        given = inputs(7, seed)
+        assert all(torch.equal(s, t) for s, t in zip(recorded(*given), step(*given)))
+
+
+def test_a_traced_network_computes_what_it_traced():
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.first, self.norm, self.last = torch.nn.Linear(24, 20), ROF_LayerNorm(20, relu=True, dropout=0.4), torch.nn.Linear(20, 5)
+
+        def forward(self, x):
+            return self.last(self.norm(self.first(x)))
+
+    net = Net().cuda().eval()
+    with torch.no_grad():
+        traced = through_a_file(torch.jit.trace(net, (rows(7, 24, 1),)))
+        assert torch.equal(traced(rows(9, 24, 2)), net(rows(9, 24, 2)))
+
+
+def test_torch_funcs_transforms_are_refused():
+    x, (w, b), rng = rows(6, 8, 1), params(8, 2), rng_tensor()
+    calls = [lambda x, w, b: layer_norm(x, w, b), lambda x, w, b: layer_norm(x, w, b, dropout=0.5, rng=rng)]
+    for call in calls:
+        for i in range(3):
+            with pytest.raises(RofError, match="transforms"):
+                torch.func.grad(lambda *t: call(*t).sum(), argnums=i)(x, w.detach(), b.detach())
+        with pytest.raises(RofError, match="transforms"):
+            torch.vmap(lambda w: call(x, w, b))(w.detach()[None])
+    with pytest.raises(RofError, match="transforms"):
+        torch.vmap(lambda r: dropout(x, 0.5, r))(rng[None])
+    with pytest.raises(RofError, match="transforms"):
+        torch.vmap(lambda s: ROF_DropoutState.next(type("S", (), {"state": s})()))(rng[None])
