@@ -15,8 +15,8 @@ Both models take two keyword arguments that upstream does not have:
     dropout_seed=int    dropout from a counter-based generator whose mask is never stored (row_ops.dropout) in place of
                         torch.nn.Dropout; the generator's state is a buffer of the model
 With both and a ReLU (or no activation), norm, activation and dropout of a hidden layer are one pass over its rows each way.
-A forward pass with dropout_seed moves the model's state on, so it must not be run again for its own backward pass
-(activation checkpointing of the whole model).
+A forward pass with dropout_seed moves the model's state on, so it cannot be run again for its own backward pass
+(activation checkpointing of the whole model): that raises RofError.
 """
 from __future__ import annotations
 

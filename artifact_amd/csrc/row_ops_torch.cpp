@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <cmath>
@@ -326,8 +327,17 @@ Tensor layer_norm_autograd(const Tensor &x, const std::optional<Tensor> &weight_
     return out;
 }
 
+// A checkpointed function's second pass runs within the backward pass: its masks would not be the first one's, and the
+// gradients wrong.
+void check_no_backward() {
+    require(torch::autograd::get_current_graph_task_id() == -1,
+            "the dropout state cannot move on during a backward pass: a checkpointed function takes the values of next() as an "
+            "argument, and a model with dropout_seed is not checkpointed as a whole");
+}
+
 // The values of one step, and the state moved on behind it.
 Tensor dropout_state_next_cuda(const Tensor &state, int64_t calls) {
+    check_no_backward();
     require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous(),
             "the dropout state must be a contiguous int64 tensor {seed, offset}");
     require(calls >= 0, "calls must not be negative");
@@ -354,6 +364,7 @@ Tensor dropout(const Tensor &x, double p, const std::optional<Tensor> &rng, int6
     return dropout_op().call(x, p, rng, call);
 }
 Tensor dropout_state_next(const Tensor &state, int64_t calls) {
+    check_no_backward();
     require(state.is_cuda(), "the dropout state must be on the GPU (move the module there)");
     check_plain(state);
     return dropout_state_next_op().call(state, calls);

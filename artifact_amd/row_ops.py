@@ -61,7 +61,8 @@ class ROF_DropoutState(torch.nn.Module):
     model, so that a resumed run draws the masks that the interrupted one would have).  `next(calls)` returns the values of
     one step and moves the offset on by `calls`; both happen on the device, so a captured step draws new masks whenever it
     is replayed.  Ranks that train together need seeds of their own (and no broadcast of buffers).  A checkpointed function
-    must be given the values, not call `next` itself: its second pass would draw other masks."""
+    must be given the values, not call `next` itself: its second pass would draw other masks, so `next` raises RofError
+    during a backward pass."""
 
     def __init__(self, seed):
         super().__init__()

@@ -3,9 +3,13 @@ import io
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from artifact_amd._lib import RofError
+from artifact_amd.ROF_models import ROF_GCN
+from artifact_amd.graphgen import features, make_workload
+from artifact_amd.reuse_conv import build_input_info
 from artifact_amd.row_ops import ROF_DropoutState, ROF_LayerNorm, dropout, layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -23,6 +27,14 @@ def params(f, seed):
 
 def rng_tensor(seed=5, offset=3):
     return torch.tensor([seed, offset], device="cuda")
+
+
+def model_on_a_graph(**kw):
+    ip, ix = make_workload("c1", 5)
+    info = build_input_info(ip, ix, 3, device="cuda", min_consumers=2)
+    torch.manual_seed(5)
+    model = ROF_GCN(24, 20, 5, 2, torch.relu, 0.4, reuse_size=info.reuse_size, kernel_type="ROF_v2", **kw).cuda()
+    return model, info, torch.from_numpy(features(len(ip) - 1, 24, seed=1)).cuda()
 
 
 def through_a_file(traced):
@@ -55,16 +67,17 @@ def test_a_traced_program_checks_what_it_is_given():
                 traced(bad)
 
 
+class Tail(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.norm = ROF_LayerNorm(24, relu=True, dropout=0.5)
+        self.state = ROF_DropoutState(3)
+
+    def forward(self, x):
+        return self.norm(x, self.state.next(2), call=1)
+
+
 def test_a_traced_module_draws_new_masks():
-    class Tail(torch.nn.Module):
-        def __init__(self):
-            super().__init__()
-            self.norm = ROF_LayerNorm(24, relu=True, dropout=0.5)
-            self.state = ROF_DropoutState(3)
-
-        def forward(self, x):
-            return self.norm(x, self.state.next(2), call=1)
-
     m, other = Tail().cuda(), Tail().cuda()
     x = rows(40, 24, 2)
     with torch.no_grad():
@@ -123,3 +136,28 @@ def test_torch_funcs_transforms_are_refused():
         torch.vmap(lambda r: dropout(x, 0.5, r))(rng[None])
     with pytest.raises(RofError, match="transforms"):
         torch.vmap(lambda s: ROF_DropoutState.next(type("S", (), {"state": s})()))(rng[None])
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+@pytest.mark.parametrize("norm", ["layer", None])
+def test_a_checkpointed_model_that_would_draw_other_masks_is_refused(norm, reentrant):
+    model, info, x = model_on_a_graph(norm=norm, dropout_seed=3)
+    x.requires_grad_(True)
+    y = torch.utils.checkpoint.checkpoint(model, x, info, use_reentrant=reentrant)
+    with pytest.raises(RofError, match="backward pass"):
+        y.sum().backward()
+    model.eval()                                             # no masks, no matter
+    y = torch.utils.checkpoint.checkpoint(model, x, info, use_reentrant=reentrant)
+    got, = torch.autograd.grad(model(x, info).sum(), x)
+    x.grad = None
+    y.sum().backward()
+    assert torch.equal(x.grad, got)
+
+
+def test_a_checkpointed_traced_module_that_would_draw_other_masks_is_refused():
+    x = rows(9, 24, 1).requires_grad_(True)
+    with torch.no_grad():
+        traced = torch.jit.trace(Tail().cuda(), (x.detach(),), check_trace=False)
+    y = torch.utils.checkpoint.checkpoint(traced, x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="backward pass"):
+        y.sum().backward()
