@@ -43,9 +43,11 @@ def _add_tails(model, widths, activation, rate, norm, dropout_seed):
 def _run_layers(model, h, inputInfo, activated):
     """The layers and what is between them.  `activated`: the hidden layers apply the activation themselves."""
     last = len(model.layers) - 1
-    counted = model.dropout_state is not None
+    # a model that was pickled whole before it could have them has neither
+    norms, state = getattr(model, "norms", None), getattr(model, "dropout_state", None)
+    counted = state is not None
     rate = model.dropout.p if counted and model.dropout.training else 0.0
-    rng = model.dropout_state.next(last) if rate and last else None    # the values of this forward pass
+    rng = state.next(last) if rate and last else None                   # the values of this forward pass
     dropped = True                                                      # what the next layer reads is ready for it
     for i, layer in enumerate(model.layers):
         if not dropped:
@@ -55,8 +57,8 @@ def _run_layers(model, h, inputInfo, activated):
             break
         dropped = False
         activation = None if activated else model.activation
-        if model.norms is not None:
-            norm, whole = model.norms[i], activation is None or activation in _RELUS
+        if norms is not None:
+            norm, whole = norms[i], activation is None or activation in _RELUS
             dropped = whole and counted
             h = layer_norm(h, norm.weight, norm.bias, eps=norm.eps, relu=whole and activation is not None,
                            dropout=rate if dropped else 0.0, rng=rng, call=i)

@@ -4,6 +4,7 @@ import torch
 
 from artifact_amd import rof_module
 from artifact_amd._lib import RofError
+from artifact_amd.ROF_models import ROF_GCN, ROF_GIN
 from artifact_amd.row_ops import ROF_DropoutState
 
 
@@ -31,3 +32,31 @@ def test_the_state_does_not_move_on_during_a_backward_pass():
     x = torch.ones(3, requires_grad=True)
     with pytest.raises(RofError, match="backward pass"):
         AsACheckpoint.apply(x).sum().backward()
+
+
+class Times(torch.nn.Module):
+    """A convolution's place in a model, without a graph or a GPU."""
+
+    def __init__(self, factor):
+        super().__init__()
+        self.factor = factor
+
+    def forward(self, x, info):
+        return x * self.factor
+
+
+def model_without_graph(cls=ROF_GCN, layers=2, rate=0.4, **kw):
+    kw = {"activation": torch.tanh} | kw
+    model = cls(6, 6, 6, layers if cls is ROF_GCN else layers + 1, dropout=rate, **kw)
+    model.layers = torch.nn.ModuleList(Times(2.0) for _ in range(layers + 1))
+    return model
+
+
+@pytest.mark.parametrize("cls", [ROF_GCN, ROF_GIN])
+def test_a_model_pickled_before_norms_and_states_still_runs(cls):
+    model = model_without_graph(cls).eval()
+    x = torch.linspace(-1, 1, 12).reshape(2, 6)
+    want = model(x, None)
+    for name in ("norms", "dropout_state"):      # what such an object does not have
+        del model.__dict__[name]
+    assert torch.equal(model(x, None), want) and torch.equal(want, torch.tanh(torch.tanh(x * 2) * 2) * 2)
