@@ -15,6 +15,9 @@ Both models take two keyword arguments that upstream does not have:
     dropout_seed=int    dropout from a counter-based generator whose mask is never stored (row_ops.dropout) in place of
                         torch.nn.Dropout; the generator's state is a buffer of the model
 With both and a ReLU (or no activation), norm, activation and dropout of a hidden layer are one pass over its rows each way.
+It is the norm that is called for it, so its hooks and wrappers take part, and its output is that of the whole pass.  A norm
+that was replaced by another module, or given a ReLU or a dropout of its own, and a dropout that was replaced or has hooks,
+run by themselves.
 A forward pass with dropout_seed moves the model's state on, so it cannot be run again for its own backward pass
 (activation checkpointing of the whole model): that raises RofError.
 """
@@ -23,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from .reuse_conv import ROF_GCNConv, ROF_GINConv, ROF_inputInfo  # noqa: F401  (re-exported like upstream)
-from .row_ops import ROF_Dropout, ROF_DropoutState, ROF_LayerNorm, layer_norm
+from .row_ops import ROF_Dropout, ROF_DropoutState, ROF_LayerNorm
 
 __all__ = ["ROF_GCN", "ROF_GIN", "ROF_inputInfo"]
 
@@ -40,14 +43,27 @@ def _add_tails(model, widths, activation, rate, norm, dropout_seed):
     model.dropout_state = None if dropout_seed is None else ROF_DropoutState(dropout_seed)
 
 
+def _takes_more(norm):
+    """Whether the pass of this norm may hold the model's activation and dropout as well."""
+    return type(norm).forward is ROF_LayerNorm.forward and not norm.relu and not norm.p
+
+
+def _can_be_part(dropout):
+    """Whether this dropout may run inside the pass of a norm: not one with hooks or a wrapper, which would not be called there."""
+    return type(dropout).forward is ROF_Dropout.forward and not (
+        "forward" in vars(dropout) or dropout._forward_hooks or dropout._forward_pre_hooks or dropout._backward_hooks or dropout._backward_pre_hooks)
+
+
 def _run_layers(model, h, inputInfo, activated):
     """The layers and what is between them.  `activated`: the hidden layers apply the activation themselves."""
     last = len(model.layers) - 1
     # a model that was pickled whole before it could have them has neither
     norms, state = getattr(model, "norms", None), getattr(model, "dropout_state", None)
-    counted = state is not None
+    counted = state is not None and isinstance(model.dropout, ROF_Dropout)
     rate = model.dropout.p if counted and model.dropout.training else 0.0
-    rng = state.next(last) if rate and last else None                   # the values of this forward pass
+    # the values of this forward pass; norms that drop by themselves use the calls behind the model's own
+    own = norms is not None and any(isinstance(norm, ROF_LayerNorm) and norm.p and norm.training for norm in norms)
+    rng = state.next(2 * last if own else last) if state is not None and (rate or own) and last else None
     dropped = True                                                      # what the next layer reads is ready for it
     for i, layer in enumerate(model.layers):
         if not dropped:
@@ -59,10 +75,14 @@ def _run_layers(model, h, inputInfo, activated):
         activation = None if activated else model.activation
         if norms is not None:
             norm, whole = norms[i], activation is None or activation in _RELUS
-            dropped = whole and counted
-            h = layer_norm(h, norm.weight, norm.bias, eps=norm.eps, relu=whole and activation is not None,
-                           dropout=rate if dropped else 0.0, rng=rng, call=i)
-            activation = None if whole else activation
+            if _takes_more(norm):
+                dropped = whole and counted and _can_be_part(model.dropout)
+                h = norm(h, rng, call=i, relu=whole and activation is not None, dropout=rate if dropped else 0.0)
+                activation = None if whole else activation
+            elif isinstance(norm, ROF_LayerNorm):
+                h = norm(h, rng, call=last + i)
+            else:
+                h = norm(h)
         if activation is not None:
             h = activation(h)
     return h

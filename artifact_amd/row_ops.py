@@ -112,8 +112,11 @@ class ROF_LayerNorm(torch.nn.Module):
         if self.bias is not None:
             torch.nn.init.zeros_(self.bias)
 
-    def forward(self, x, rng=None, call=0, out_dtype=None):
-        return layer_norm(x, self.weight, self.bias, eps=self.eps, relu=self.relu, dropout=self.p if self.training else 0.0,
+    def forward(self, x, rng=None, call=0, out_dtype=None, relu=None, dropout=None):
+        """`relu` and `dropout` (a rate, whatever the mode), where given, stand for the module's own."""
+        if dropout is None:
+            dropout = self.p if self.training else 0.0
+        return layer_norm(x, self.weight, self.bias, eps=self.eps, relu=self.relu if relu is None else relu, dropout=dropout,
                           rng=rng, call=call, out_dtype=out_dtype)
 
     def extra_repr(self):

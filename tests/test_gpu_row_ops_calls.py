@@ -29,11 +29,11 @@ def rng_tensor(seed=5, offset=3):
     return torch.tensor([seed, offset], device="cuda")
 
 
-def model_on_a_graph(**kw):
+def model_on_a_graph(activation=torch.relu, **kw):
     ip, ix = make_workload("c1", 5)
     info = build_input_info(ip, ix, 3, device="cuda", min_consumers=2)
     torch.manual_seed(5)
-    model = ROF_GCN(24, 20, 5, 2, torch.relu, 0.4, reuse_size=info.reuse_size, kernel_type="ROF_v2", **kw).cuda()
+    model = ROF_GCN(24, 20, 5, 2, activation, 0.4, reuse_size=info.reuse_size, kernel_type="ROF_v2", **kw).cuda()
     return model, info, torch.from_numpy(features(len(ip) - 1, 24, seed=1)).cuda()
 
 
@@ -161,3 +161,58 @@ def test_a_checkpointed_traced_module_that_would_draw_other_masks_is_refused():
     y = torch.utils.checkpoint.checkpoint(traced, x, use_reentrant=False)
     with pytest.raises(RuntimeError, match="backward pass"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("activation", [torch.relu, torch.tanh])
+def test_the_models_call_their_norms(activation):
+    """Hooks, pre-hooks and wrappers of a norm take part, and what they change is what the model computes with."""
+    model, info, x = model_on_a_graph(norm="layer", dropout_seed=3, activation=activation)
+    want, seen = model(x, info), []
+    model.dropout_state.state.copy_(torch.tensor([3, 0]))
+    handles = [n.register_forward_hook(lambda m, args, out: seen.append(out.shape)) for n in model.norms]
+    assert torch.equal(model(x, info), want) and seen == [(len(x), 20)] * 2
+    for h in handles:
+        h.remove()
+    weight = torch.linspace(0.5, 1.5, 20, device="cuda")
+
+    def gather(m, args):
+        m.weight.data.copy_(weight)
+
+    model.norms[0].register_forward_pre_hook(gather)
+    model.dropout_state.state.copy_(torch.tensor([3, 0]))
+    got = model(x, info)
+    assert not torch.equal(got, want)
+    model.dropout_state.state.copy_(torch.tensor([3, 0]))
+    other, _, _ = model_on_a_graph(norm="layer", dropout_seed=3, activation=activation)
+    other.norms[0].weight.data.copy_(weight)
+    assert torch.equal(other(x, info), got)
+    torch.nn.utils.parametrizations.weight_norm(model.norms[1], dim=None)
+    model(x, info).sum().backward()
+    assert model.norms[1].parametrizations.weight.original0.grad is not None
+
+
+def test_the_models_call_a_dropout_with_hooks():
+    model, info, x = model_on_a_graph(norm="layer", dropout_seed=3)
+    want, seen = model(x, info), []
+    model.dropout_state.state.copy_(torch.tensor([3, 0]))
+    model.dropout.register_forward_hook(lambda m, args, out: seen.append((args[0], out)))
+    got = model(x, info)
+    assert len(seen) == 2 and model.dropout_state.state.tolist() == [3, 2]
+    rng = rng_tensor(3, 0)
+    for i, (given, out) in enumerate(seen):
+        assert torch.equal(out, dropout(given, 0.4, rng, call=i))
+    # The same masks and sums, but the scale behind the norm's rounding, not in its parameters: 5 roundings of 2^-24 of values
+    # up to 2 (3 + 0.3), which the next layer's 20 products and its norm (up to 4) magnify less than 100 times: below 2e-4
+    assert torch.allclose(got, want, rtol=0, atol=2e-4)
+
+
+def test_a_models_norm_with_a_relu_or_a_dropout_of_its_own():
+    model, info, x = model_on_a_graph(norm="layer", dropout_seed=3, activation=torch.tanh)
+    model.norms[0].relu, model.norms[1].p = True, 0.25
+    got = model(x, info)
+    assert model.dropout_state.state.tolist() == [3, 4]
+    rng, h = rng_tensor(3, 0), x
+    for i, (layer, norm) in enumerate(zip(model.layers, model.norms)):
+        h = layer_norm(layer(h, info), norm.weight, norm.bias, relu=i == 0, dropout=0.25 if i else 0.0, rng=rng, call=2 + i)
+        h = dropout(torch.tanh(h), 0.4, rng, call=i)
+    assert torch.equal(model.layers[2](h, info), got)

@@ -60,3 +60,26 @@ def test_a_model_pickled_before_norms_and_states_still_runs(cls):
     for name in ("norms", "dropout_state"):      # what such an object does not have
         del model.__dict__[name]
     assert torch.equal(model(x, None), want) and torch.equal(want, torch.tanh(torch.tanh(x * 2) * 2) * 2)
+
+
+def test_a_replaced_norm_or_dropout_is_called_by_itself():
+    x = torch.linspace(-1, 1, 12).reshape(2, 6) ** 3
+    model = model_without_graph(activation=torch.relu, norm="layer", rate=0.0)
+    model.norms = torch.nn.ModuleList(torch.nn.LayerNorm(6) for _ in range(2))
+    want = torch.nn.functional.layer_norm
+    assert torch.equal(model(x, None), torch.relu(want(torch.relu(want(x * 2, (6,))) * 2, (6,))) * 2)
+    seen = []
+
+    class Mine(torch.nn.Module):
+        def forward(self, h):
+            seen.append(h)
+            return h + 1
+
+    for norm in (None, "layer"):
+        model = model_without_graph(norm=norm, dropout_seed=3)       # a state on the CPU: nothing may ask it for values
+        if norm:
+            model.norms = torch.nn.ModuleList(torch.nn.Identity() for _ in range(2))
+        model.dropout = Mine()
+        assert torch.equal(model(x, None), (torch.tanh((torch.tanh(x * 2) + 1) * 2) + 1) * 2)
+        assert len(seen) == 2 and torch.equal(seen[0], torch.tanh(x * 2))
+        seen.clear()
