@@ -85,7 +85,8 @@ void check_param(const char *name, const Tensor &t, const Tensor &x) {
 void check_rate(double p) { require(p >= 0.0 && p <= 1.0, "a dropout rate must lie between 0 and 1"); }
 void check_rng(const Tensor &rng, const Tensor &x) {
     require(rng.defined(), "dropout needs rng: an int64 tensor {seed, offset} on the device of x (see ROF_DropoutState)");
-    require(rng.scalar_type() == at::kLong && rng.device() == x.device() && rng.numel() == 2 && rng.is_contiguous(),
+    require(rng.scalar_type() == at::kLong && rng.device() == x.device() && rng.numel() == 2 && rng.is_contiguous() &&
+                !rng.is_neg(),
             "rng must be a contiguous int64 tensor of two elements {seed, offset} on the device of x");
 }
 
@@ -338,7 +339,7 @@ void check_no_backward() {
 // The values of one step, and the state moved on behind it.
 Tensor dropout_state_next_cuda(const Tensor &state, int64_t calls) {
     check_no_backward();
-    require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous(),
+    require(state.scalar_type() == at::kLong && state.numel() == 2 && state.is_contiguous() && !state.is_neg(),
             "the dropout state must be a contiguous int64 tensor {seed, offset}");
     require(calls >= 0, "calls must not be negative");
     const c10::DeviceGuard guard(state.device());

@@ -216,3 +216,12 @@ def test_a_models_norm_with_a_relu_or_a_dropout_of_its_own():
         h = layer_norm(layer(h, info), norm.weight, norm.bias, relu=i == 0, dropout=0.25 if i else 0.0, rng=rng, call=2 + i)
         h = dropout(torch.tanh(h), 0.4, rng, call=i)
     assert torch.equal(model.layers[2](h, info), got)
+
+
+def test_a_generator_state_with_the_negative_bit_is_refused():
+    x, rng = rows(6, 8, 1), rng_tensor()
+    state = ROF_DropoutState(3).cuda()
+    state.state = state.state._neg_view()
+    for call in (lambda: dropout(x, 0.5, rng._neg_view()), lambda: layer_norm(x, dropout=0.5, rng=rng._neg_view()), state.next):
+        with pytest.raises(RofError, match="contiguous int64"):
+            call()
