@@ -346,13 +346,34 @@ struct Param {
             for (int e = 0; e < V; ++e) {
                 if (m.has(j, e)) most = fmaxf(most, fabsf(t[j][e]));
                 t[j][e] *= factor;
-                if (!kLds) v[j][e] = t[j][e];
             }
-            if (kLds) {
+            set(j, t[j]);
+        }
+    }
+    // For a bias of which only the sign of h w + bias matters, as in the backward kernel: where the weight is zero that is the
+    // bias's own sign, which an infinity has as well.  Such a column is then never near the border, where one with a weight and
+    // a bias of zero would take every row through the 64-bit statistics (2^22 x 256 bfloat16 with ReLU and dropout and one such
+    // column: 1974 us, without it 1152).
+    template <typename W>
+    __device__ __forceinline__ void decide(const W &weight) {
 #pragma unroll
-                for (int i = 0; i < Q; ++i)
-                    lds[(j * Q + i) * Map::LANES] = make_float4(t[j][4 * i], t[j][4 * i + 1], t[j][4 * i + 2], t[j][4 * i + 3]);
-            }
+        for (int j = 0; j < K; ++j) {
+            float w[V], b[V];
+            weight.get(j, w);
+            get(j, b);
+#pragma unroll
+            for (int e = 0; e < V; ++e) b[e] = w[e] != 0.f ? b[e] : b[e] > 0.f ? __builtin_inff() : -__builtin_inff();
+            set(j, b);
+        }
+    }
+    __device__ __forceinline__ void set(int j, const float (&from)[V]) {
+        if constexpr (kLds) {
+#pragma unroll
+            for (int i = 0; i < Q; ++i)
+                lds[(j * Q + i) * Map::LANES] = make_float4(from[4 * i], from[4 * i + 1], from[4 * i + 2], from[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] = from[e];
         }
     }
     __device__ __forceinline__ void get(int j, float (&to)[V]) const {
@@ -532,7 +553,8 @@ __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd
     float dw[K][V], db[K][V], wmost, bmost;
     const Param<Map, true> weight(m, a.weight, 1.f, 0.f, wstore, wmost);
     // in columns that do not exist pre is -infinity: never near the border, and the gate is closed
-    const ParamOf<Map, RELU> bias(m, a.bias, 0.f, -__builtin_inff(), bstore, bmost);
+    ParamOf<Map, RELU> bias(m, a.bias, 0.f, -__builtin_inff(), bstore, bmost);
+    if constexpr (RELU) bias.decide(weight);
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll

@@ -225,3 +225,22 @@ def test_a_generator_state_with_the_negative_bit_is_refused():
     for call in (lambda: dropout(x, 0.5, rng._neg_view()), lambda: layer_norm(x, dropout=0.5, rng=rng._neg_view()), state.next):
         with pytest.raises(RofError, match="contiguous int64"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("f", [3, 7, 47, 100, 256, 700, 1500, 4099, 7001])
+def test_columns_without_a_weight_pass_the_gate_by_their_biass_sign(f, dtype):
+    """Also where it is as small as numbers get, or zero, in the last column too; the others pass as ever."""
+    n = 37
+    x, (w, b), dy = rows(n, f, 1, dtype), params(f, 2), torch.ones(n, f, device="cuda")
+    signs = torch.tensor([0.0, -0.0, 1e-40, -1e-40, 1e-9, -1e-9, 2.0, -2.0], device="cuda")
+    at = torch.arange(f - 1, -1, -max(1, f // 8), device="cuda")[:8]
+    for zero in (0.0, -0.0):
+        with torch.no_grad():
+            w[at], b[at] = zero, signs[:len(at)]
+        h = x.double() - x.double().mean(1, keepdim=True)
+        h = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+        gate = h * w.detach().double() + b.detach().double() > 0
+        db, = torch.autograd.grad(layer_norm(x, w, b, relu=True, out_dtype=torch.float32), b, dy)
+        assert torch.equal(db.double(), gate.double().sum(0))       # whole numbers; every sign is settled in 64 bits
+        assert torch.equal(db[at] > 0, signs[:len(at)] > 0)
