@@ -244,3 +244,36 @@ def test_columns_without_a_weight_pass_the_gate_by_their_biass_sign(f, dtype):
         db, = torch.autograd.grad(layer_norm(x, w, b, relu=True, out_dtype=torch.float32), b, dy)
         assert torch.equal(db.double(), gate.double().sum(0))       # whole numbers; every sign is settled in 64 bits
         assert torch.equal(db[at] > 0, signs[:len(at)] > 0)
+
+
+def test_calls_on_a_busy_stream_wait_for_what_is_before_them():
+    """Everything is on the device beforehand, so that nothing on the host waits for the stream: a kernel on any other stream
+    would read the rows that the copy at the end of the queue is about to replace."""
+    side = torch.cuda.Stream()
+    w, b = params(64, 2)
+    old, new, dy, rng = rows(50, 64, 1), rows(50, 64, 2), rows(50, 64, 3), rng_tensor()
+    big = torch.randn(4096, 4096, device="cuda")
+    state = ROF_DropoutState(8).cuda()
+
+    def calls(x):
+        used = state.next(2)
+        y = layer_norm(x, w, b, relu=True, dropout=0.5, rng=rng)
+        return (y.detach(), used, dropout(x.detach(), 0.5, used)) + torch.autograd.grad(y, (x, w, b), dy)
+
+    calls(old.clone().requires_grad_(True))              # kernels loaded, streams made
+    want = calls(new.clone().requires_grad_(True))
+    state.state.fill_(0)
+    x, at = old.clone().requires_grad_(True), torch.tensor([8, 2], device="cuda")
+    with torch.cuda.stream(side):
+        big @ big
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            out = big @ big                              # tens of milliseconds
+        x.detach().copy_(new)
+        state.state.copy_(at)
+        got = calls(x)
+        busy = not side.query()
+    torch.cuda.synchronize()
+    assert busy and out.shape == big.shape
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
