@@ -17,7 +17,7 @@ using namespace rofn;
 // kManyRounds rounds of work on it is tiles of four rounds, see norm_blocks, else workgroups that stay.
 constexpr int kBackwardBlocks = 1280, kBackwardTiles = 16384;
 constexpr int64_t kSomeRounds = 65536, kManyRounds = 100000;
-constexpr int kTiledColumns = 512;   // rows of more columns are several vectors per lane of a whole wavefront in either type
+constexpr int kTiledColumns = 512;   // rows of more columns are more than 64 vectors in either type
 constexpr int kParamsChunks = 128;   // rows that the first of two passes leaves of so many partial ones
 // An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
 constexpr int64_t kStreamOutBytes = 128 << 20;
@@ -195,6 +195,12 @@ NormShape norm_shape(int f, int x_dtype) {
     return {c->lpr, c->waves, c->k, false};
 }
 
+// Up to 64 vectors, in whichever of the shapes.
+bool is_lean(const NormShape &s) { return s.waves * s.lpr * s.k <= 64; }
+int64_t rounds_of(const NormShape &s, int64_t n) { return (n + s.rows() - 1) / s.rows(); }
+// Whether the backward launch is tiles, see norm_blocks.
+bool is_tiled(const NormShape &s, int64_t n) { return is_lean(s) && rounds_of(s, n) >= kManyRounds; }
+
 // How many workgroups, and which rounds each takes.
 // Forward: a workgroup per four adjacent rounds where that makes thousands of them (2^22 x 256 bfloat16: 743 us against 862
 // with 2048 workgroups that stay and step through the matrix together; 10^6 x 100 float32 142 / 155), else as many as stay:
@@ -209,8 +215,8 @@ NormShape norm_shape(int f, int x_dtype) {
 // with 1024 workgroups: 77 us, with 1280 82) and two in wide rows (20011 x 4099 bfloat16 with four wavefronts: 106 us against
 // 117 one at a time; forward with three 62 / 71).
 int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
-    const int64_t rows = s.rows(), rounds = (a.n + rows - 1) / rows;
-    const bool lean = s.waves * s.lpr * s.k <= 64, f32 = x_dtype == ROF_F32;   // lean: up to 64 vectors, see kTiledColumns
+    const int64_t rows = s.rows(), rounds = rounds_of(s, a.n);
+    const bool lean = is_lean(s), f32 = x_dtype == ROF_F32;
     int64_t most;
     if (!backward && rounds / 4 >= 4096 && rounds / 4 < kMostBlocks) {
         a.inner = 4;
@@ -220,7 +226,7 @@ int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
         most = lean ? 2048 : 1024;
     } else if (lean) {
         a.inner = rounds >= kSomeRounds ? 4 : 1;
-        most = rounds >= kManyRounds ? (f32 ? kBackwardTiles : kBackwardTiles / 4) : rounds >= kSomeRounds && f32 && s.k == 1 ? 1280 : 1024;
+        most = is_tiled(s, a.n) ? (f32 ? kBackwardTiles : kBackwardTiles / 4) : rounds >= kSomeRounds && f32 && s.k == 1 ? 1280 : 1024;
     } else {
         a.inner = rounds < 2048 ? 1 : 2;
         most = s.waves == 2 || s.lpr < 64 ? 1024 : 512;
@@ -354,7 +360,9 @@ int rof_layer_norm(const void *x, int x_dtype, int64_t ldx, int64_t n, int f, co
 
 size_t rof_layer_norm_backward_workspace_bytes(int64_t n, int f) {
     if (n <= 0 || f <= 0) return 0;
-    const int64_t rows = n >= kManyRounds && f <= kTiledColumns ? kBackwardTiles + kParamsChunks : std::min<int64_t>(n, kBackwardBlocks);
+    // for rows of either type
+    const bool tiled = f <= kTiledColumns && (is_tiled(norm_shape(f, ROF_F32), n) || is_tiled(norm_shape(f, ROF_BF16), n));
+    const int64_t rows = tiled ? kBackwardTiles + kParamsChunks : std::min<int64_t>(n, kBackwardBlocks);
     return (size_t)rows * 2 * (size_t)f * sizeof(float);
 }
 

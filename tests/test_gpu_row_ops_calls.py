@@ -1,4 +1,5 @@
 """How the row operators are called on the GPU: recorded programs, other streams, wrapped tensors."""
+import ctypes as C
 import io
 
 import pytest
@@ -6,7 +7,8 @@ import torch
 import torch.utils.checkpoint
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from artifact_amd._lib import RofError
+from artifact_amd import _lib
+from artifact_amd._lib import DropoutOpts, RofError
 from artifact_amd.ROF_models import ROF_GCN
 from artifact_amd.graphgen import features, make_workload
 from artifact_amd.reuse_conv import build_input_info
@@ -277,3 +279,22 @@ def test_calls_on_a_busy_stream_wait_for_what_is_before_them():
     torch.cuda.synchronize()
     assert busy and out.shape == big.shape
     assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype,f,n", [(torch.bfloat16, 512, 399996), (torch.bfloat16, 512, 399997), (torch.float32, 512, 399997),
+                                       (torch.float32, 256, 399996), (torch.float32, 256, 399997), (torch.bfloat16, 16, 100000),
+                                       (torch.float32, 5, 12799872), (torch.float32, 5, 12799873), (torch.bfloat16, 5, 12799873)])
+def test_the_backward_launch_stays_in_its_workspace(dtype, f, n):
+    L, st, kind = _lib.lib(), torch.cuda.current_stream().cuda_stream, 0 if dtype == torch.float32 else 1
+    x = torch.randn(n, f, device="cuda", dtype=dtype)
+    dy, (w, b), rng = x.flip(0), params(f, 2), rng_tensor()
+    dx, dw, db = torch.empty_like(x), torch.empty(f, device="cuda"), torch.empty(f, device="cuda")
+    size = L.rof_layer_norm_backward_workspace_bytes(n, f)
+    ws = torch.full((size // 4 + 4096,), -7.0, device="cuda")
+    opts = C.byref(DropoutOpts(0.5, rng.data_ptr(), 0))
+    assert L.rof_layer_norm_backward(dy.data_ptr(), kind, f, x.data_ptr(), kind, f, n, f, w.data_ptr(), b.data_ptr(), 1e-5, 1, opts,
+                                     dx.data_ptr(), f, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), size, st) == 0
+    assert (ws[size // 4:] == -7).all()
+    xx = x.requires_grad_(True)
+    want = torch.autograd.grad(layer_norm(xx, w, b, relu=True, dropout=0.5, rng=rng), (xx, w, b), dy)
+    assert all(torch.equal(s, t) for s, t in zip((dx, dw, db), want))

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from artifact_amd import rof_module
+from artifact_amd import _lib, rof_module
 from artifact_amd._lib import RofError
 from artifact_amd.ROF_models import ROF_GCN, ROF_GIN
 from artifact_amd.row_ops import ROF_DropoutState
@@ -83,3 +83,12 @@ def test_a_replaced_norm_or_dropout_is_called_by_itself():
         assert torch.equal(model(x, None), (torch.tanh((torch.tanh(x * 2) + 1) * 2) + 1) * 2)
         assert len(seen) == 2 and torch.equal(seen[0], torch.tanh(x * 2))
         seen.clear()
+
+
+@pytest.mark.parametrize("f,n", [(512, 399997), (300, 1599985), (256, 399997), (47, 1599985), (5, 12799873), (1, 25599745)])
+def test_the_workspace_grows_where_the_launch_becomes_tiles(f, n):
+    """From 100000 rounds of rows on, which are 4 to 256 rows by width and type: n is the first such number of rows in the type
+    with fewer rows a round.  Before that a row per workgroup that can stay, 1280."""
+    size = _lib.lib().rof_layer_norm_backward_workspace_bytes
+    assert size(100000, f) == size(n - 1, f) == 1280 * 2 * f * 4
+    assert size(n, f) == (16384 + 128) * 2 * f * 4
