@@ -14,9 +14,9 @@ namespace {
 using namespace rofn;
 
 // Workgroups of the backward launch at most: each leaves a row of 2 f partial sums for the parameters' gradients.  From
-// kManyRounds rounds of work on it is tiles of four rounds, see norm_blocks, else workgroups that stay.
+// kManyRounds rounds of work on it is tiles of four rounds, else workgroups that stay; all of these: see norm_blocks.
 constexpr int kBackwardBlocks = 1280, kBackwardTiles = 16384;
-constexpr int64_t kSomeRounds = 65536, kManyRounds = 100000;
+constexpr int64_t kPairedRounds = 20000, kFullRounds = 30000, kManyRounds = 100000;
 constexpr int kTiledColumns = 512;   // rows of more columns are more than 64 vectors in either type
 constexpr int kParamsChunks = 128;   // rows that the first of two passes leaves of so many partial ones
 // An output of this size is beyond what the 256 MB Infinity Cache keeps beside its inputs until it is read again.
@@ -208,12 +208,22 @@ bool is_tiled(const NormShape &s, int64_t n) { return is_lean(s) && rounds_of(s,
 // Backward: each workgroup leaves a row of partial sums.  With many rounds it is tiles of four adjacent ones, handed out as
 // others end: up to 16384 for float32 (10^6 x 200 424 us; 4096 tiles 471, 1280 workgroups that stay 478; 2.4 M x 100 512 / 564 /
 // 570), up to 4096 for bfloat16, whose workgroups are fewer on a CU (1.6 M x 300 602, 16384 tiles 653, 1024 that stay 602; 2.4 M x
-// 47 171 / 184 / 170; 2^22 x 256 1132 / 1119 / 1207), and more launches and traffic for their sums.  With fewer rounds as many
-// workgroups stay as fit: five on a CU where a lane holds one float32 vector (2^18 x 256 to bfloat16 122 us, with four 127;
-// 10^5 rounds are where 5 us more for the sums pay), else four, or two where the lanes hold several vectors, whose registers leave
-// room for no more; four rounds at a time (131072 rounds: 269 us, one at a time 283), but one where there are few (37500 rounds
-// with 1024 workgroups: 77 us, with 1280 82) and two in wide rows (20011 x 4099 bfloat16 with four wavefronts: 106 us against
-// 117 one at a time; forward with three 62 / 71).
+// 47 171 / 184 / 170; 2^22 x 256 1132 / 1119 / 1207), and more launches and traffic for their sums.  With fewer rounds
+// workgroups stay, as many as fit: four on a CU (1024), two (512) where a lane holds several bfloat16 vectors, whose registers
+// leave room for no more.  Rows of up to 64 vectors, a dozen widths with and without ReLU and dropout, geometric means of the
+// times against one round at a time with 1024 workgroups, by the number of rounds:
+//                                          4000  16000  20000  24000  28000  32768  50000  65536  80000  99000
+//   two adjacent rounds    float32         1.00   1.01   1.00   0.99   0.99   1.00   0.99   0.99   0.99   0.99
+//                          bfloat16        1.00   1.01   1.00   0.98   1.00   0.98   0.98   0.98   0.98   0.98
+//   four                   float32         1.08   1.02   1.02   1.01   1.02   1.01   1.00   0.99   0.98   0.98
+//                          bfloat16        1.07   1.02   1.01   1.01   1.04   0.99   0.99   0.98   0.97   0.97
+//   two, 1280 workgroups   float32         1.05   1.04   1.03   1.01   1.01   0.98   0.98   0.97   0.98   0.98
+//     two vectors a lane   float32         1.13   1.13   1.16   1.19   1.12   1.11   1.12   1.10   1.10   1.10
+//                          bfloat16        1.09   1.12   1.08   1.14   1.14   1.09   1.12   1.09   1.10   1.10
+//   two, 512 workgroups    float32         1.01   1.09   1.09   1.15   1.20   1.26   1.28   1.27   1.26   1.26
+//     three vectors a lane bfloat16        0.86   0.96   0.95   0.95   0.96   0.96   0.97   0.97   0.97   0.98
+// So two rounds from kPairedRounds on, and five workgroups on a CU for one float32 vector from kFullRounds on.  Wide rows: two
+// rounds (20011 x 4099 bfloat16 with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
 int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
     const int64_t rows = s.rows(), rounds = rounds_of(s, a.n);
     const bool lean = is_lean(s), f32 = x_dtype == ROF_F32;
@@ -225,8 +235,14 @@ int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
         a.inner = lean || rounds < 2048 ? 1 : 2;
         most = lean ? 2048 : 1024;
     } else if (lean) {
-        a.inner = rounds >= kSomeRounds ? 4 : 1;
-        most = is_tiled(s, a.n) ? (f32 ? kBackwardTiles : kBackwardTiles / 4) : rounds >= kSomeRounds && f32 && s.k == 1 ? 1280 : 1024;
+        const bool tiled = is_tiled(s, a.n);
+        a.inner = tiled ? 4 : rounds >= kPairedRounds ? 2 : 1;
+        if (tiled)
+            most = f32 ? kBackwardTiles : kBackwardTiles / 4;
+        else if (f32)
+            most = s.k == 1 && rounds >= kFullRounds ? kBackwardBlocks : 1024;
+        else
+            most = s.k == 1 ? 1024 : 512;
     } else {
         a.inner = rounds < 2048 ? 1 : 2;
         most = s.waves == 2 || s.lpr < 64 ? 1024 : 512;
