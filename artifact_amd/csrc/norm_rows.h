@@ -10,7 +10,13 @@
 // A row is held in registers from its one read to its one write, so the variance is the mean square of the differences
 // from the mean (no cancellation) at the price of one more cross-lane sum.  The backward pass keeps nothing from the
 // forward one but x itself: statistics, gate and mask are computed again, which costs fewer bytes than storing them.
-// Every launch is bounded by memory: 8 (forward) to 25 (backward) operations an element against 8 to 12 bytes of it.
+// An element is 8 (forward) to 25 (backward) operations, with dropout a quarter or an eighth of a generator's call more (14
+// wide products and twice as many other operations), against 8 and 12 bytes of float32 rows or 4 and 6 of bfloat16 ones.  Rows that are
+// part of a wavefront are bounded by memory in either type; those of several wavefronts, and of bfloat16 above 32 columns a
+// lane, by what their registers leave of wavefronts to hide the barriers and the loads behind.
+//
+// Times in this header and in row_ops.hip are of the kernel alone, events around twenty launches; figures that are compared
+// are of one run, and runs differ by up to 5 %.  A profiler's are up to 10 % longer.
 #ifndef ROF_NORM_ROWS_H_
 #define ROF_NORM_ROWS_H_
 
@@ -323,8 +329,8 @@ struct Scratch {
 
 // A lane's columns of a parameter.  In registers, but in LDS in the backward kernel of rows that are several wavefronts:
 // there a lane holds up to 32 columns, and it is registers (of the gradient's sums above all) that bound the wavefronts in
-// flight (20011 x 4099 bfloat16 with ReLU and dropout: 210 us with them in registers, 141 from LDS; without ReLU 113 either
-// way, and the forward kernel, which has registers to spare, 2 to 10 % slower from LDS).  A lane reads back only what it
+// flight (20011 x 4099 bfloat16 with ReLU and dropout: 210 us with them in registers, 141 from LDS; without ReLU no
+// difference, and the forward kernel, which has registers to spare, 2 to 10 % slower from LDS).  A lane reads back only what it
 // wrote, 16 bytes at a time in lane order, so there is neither a barrier nor a conflict.
 template <typename Map, bool BACKWARD>
 struct Param {
@@ -353,7 +359,7 @@ struct Param {
     // For a bias of which only the sign of h w + bias matters, as in the backward kernel: where the weight is zero that is the
     // bias's own sign, which an infinity has as well.  Such a column is then never near the border, where one with a weight and
     // a bias of zero would take every row through the 64-bit statistics (2^22 x 256 bfloat16 with ReLU and dropout and one such
-    // column: 1974 us, without it 1152).
+    // column: 1955 us, without it 1124).
     template <typename W>
     __device__ __forceinline__ void decide(const W &weight) {
 #pragma unroll
@@ -393,10 +399,10 @@ struct Param {
     }
 };
 
-// Forward.  A lane group works on one row while its next one is on its way; reads and writes the matrix once.  Alone on the
-// card, of the bytes it moves: 2^18 x 256 float32 99 us, 5.4 TB/s; 2.4 M x 47 float32 185 us, 4.9; 20011 x 4099 bfloat16 71 us,
-// 4.6; with ReLU and dropout 10^6 x 100 float32 151 us, 5.3; 2^22 x 256 bfloat16 820 us, 5.2 (a copy reaches 4.5 to 5.9);
-// 16384 x 16 float32 3 us, which is a launch.
+// Forward.  A lane group works on one row while its next one is on its way; reads and writes the matrix once.  Of the bytes
+// it moves: 2^18 x 256 float32 96 us, 5.6 TB/s, with ReLU 97; 2.4 M x 47 float32 182 us, 5.0; 2^20 x 128 bfloat16 to float32
+// 165 us, 4.9; 20011 x 4099 bfloat16 73 us, 4.5; with ReLU and dropout 10^6 x 100 float32 150 us, 5.3; 2^22 x 256 bfloat16
+// 740 us, 5.8 (a copy reaches 4.5 to 5.9); 16384 x 16 float32 4 us, which is a launch.
 template <typename TX, typename TY, int LPR, int WAVES, int K>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_fwd_kernel(NormArgs a) {
     using Map = RowMap<TX, LPR, WAVES, K>;
@@ -537,9 +543,11 @@ template <typename Map, bool NEEDED>
 using ParamOf = std::conditional_t<NEEDED, Param<Map, true>, NoParam>;
 
 // Backward.  As forward, with the gradient's row beside that of x: two reads and a write, and the parameters' gradients of the
-// workgroup's rows in registers up to its end.  Measured alike: 2.4 M x 47 float32 264 us, 5.1 TB/s; 2^20 x 64 bfloat16 64 us, 6.3
-// (a third of it from the Infinity Cache); 20011 x 4099 bfloat16 119 us, 4.1 (six vectors in flight per lane are what its registers hold);
-// with ReLU and dropout 10^6 x 100 float32 207 us, 5.8; 2^22 x 256 bfloat16 1228 us, 5.2; 16384 x 16 float32 4.5 us.
+// workgroup's rows in registers up to its end.  Without the parameters' gradients (with
+// them 6 to 13 us more): 2.4 M x 47 float32 247 us, 5.5 TB/s; 2^20 x 64 bfloat16 67 us, 6.0 (a third of it from the Infinity
+// Cache); 20011 x 4099 bfloat16 107 us, 4.6 (six vectors in flight per lane are what its registers hold), with ReLU and dropout
+// 137 us; with them also 10^6 x 100 float32 208 us, 5.8; 2^20 x 128 bfloat16 to float32 185 us, 5.8; 2^22 x 256 bfloat16
+// 1119 us, 5.8; 16384 x 16 float32 4.2 us.
 // Two rows ahead instead of one are no gain (2^22 x 256 bfloat16 1425 us, with one 1355, before the launch was cut into tiles).
 template <typename TX, typename TY, int LPR, int WAVES, int K, bool RELU, bool STREAM>
 __global__ __launch_bounds__((RowMap<TX, LPR, WAVES, K>::THREADS)) void norm_bwd_kernel(NormArgs a) {
