@@ -11,9 +11,9 @@
 // from the mean (no cancellation) at the price of one more cross-lane sum.  The backward pass keeps nothing from the
 // forward one but x itself: statistics, gate and mask are computed again, which costs fewer bytes than storing them.
 // An element is 8 (forward) to 25 (backward) operations, with dropout a quarter or an eighth of a generator's call more (14
-// wide products and twice as many other operations), against 8 and 12 bytes of float32 rows or 4 and 6 of bfloat16 ones.  Rows that are
-// part of a wavefront are bounded by memory in either type; those of several wavefronts, and of bfloat16 above 32 columns a
-// lane, by what their registers leave of wavefronts to hide the barriers and the loads behind.
+// wide products and twice as many other operations), against 8 and 12 bytes of float32 rows or 4 and 6 of bfloat16 ones.
+// Rows that are part of a wavefront are bounded by memory in either type; those of several wavefronts, and of several
+// bfloat16 vectors per lane, by what their registers leave of wavefronts to hide the barriers and the loads behind.
 //
 // Times in this header and in row_ops.hip are of the kernel alone, events around twenty launches; figures that are compared
 // are of one run, and runs differ by up to 5 %.  A profiler's are up to 10 % longer.

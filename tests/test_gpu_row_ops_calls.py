@@ -298,3 +298,29 @@ def test_the_backward_launch_stays_in_its_workspace(dtype, f, n):
     xx = x.requires_grad_(True)
     want = torch.autograd.grad(layer_norm(xx, w, b, relu=True, dropout=0.5, rng=rng), (xx, w, b), dy)
     assert all(torch.equal(s, t) for s, t in zip((dx, dw, db), want))
+
+
+def test_a_traced_function_is_differentiable():
+    (w, b), rng = (t.detach() for t in params(24, 1)), rng_tensor()
+
+    def call(x):
+        return dropout(layer_norm(x, w, b, relu=True), 0.5, rng)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(call, (rows(7, 24, 2),))
+    for n in (7, 11, 11, 11):                            # the interpreter specialises after its first runs
+        x, dy = rows(n, 24, n).requires_grad_(True), rows(n, 24, 5)
+        want, = torch.autograd.grad(call(x), x, dy)
+        assert torch.equal(torch.autograd.grad(traced(x), x, dy)[0], want)
+
+
+def test_a_batch_of_gradients_at_once():
+    """is_grads_batched, which jacobian(vectorize=True) uses: one call of the operator for each."""
+    x, (w, b), rng = rows(6, 8, 1).requires_grad_(True), params(8, 2), rng_tensor()
+    batch = torch.stack([rows(6, 8, s) for s in (3, 4, 5)])
+    for y, leaves in ((layer_norm(x, w, b, relu=True, dropout=0.5, rng=rng), (x, w, b)), (layer_norm(x, w, b), (w,)),
+                      (dropout(x, 0.5, rng), (x,))):
+        got = torch.autograd.grad(y, leaves, batch, is_grads_batched=True, retain_graph=True)
+        for i, dy in enumerate(batch):
+            want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            assert all(torch.equal(s[i], t) for s, t in zip(got, want))
