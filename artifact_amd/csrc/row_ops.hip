@@ -108,13 +108,15 @@ __global__ void dropout_state_next_kernel(int64_t *state, int64_t calls, int64_t
 
 // Sums of the partial rows, column by column in a fixed order: 16 columns x 64 slices of the rows per workgroup (the
 // columns are few, so narrow workgroups are what makes enough of them).  3 us (256 rows of 32) to 9 us (512 rows of 8198);
-// 1024 rows of 128 take 5 us with eight loads under way per lane, 7 with the compiler's choice.
+// 1024 rows of 128 take 5 us with eight loads under way per lane, 7 with the compiler's choice.  In 64 bits, which costs 0 to
+// 0.3 us and leaves of the gradients' error what the workgroups' own sums have (16384 x 16 float32, the bias's: 5.8e-8 of its
+// norm, in 32 bits 1.9e-7).
 __global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restrict__ partial, int blocks, int f,
                                                             float *__restrict__ dweight, float *__restrict__ dbias) {
-    __shared__ float red[64][16];
+    __shared__ double red[64][16];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     const int c = blockIdx.x * 16 + tx;
-    float s = 0.f;
+    double s = 0.0;
     if (c < 2 * f) {
 #pragma unroll 8
         for (int b = ty; b < blocks; b += 64) s += partial[(int64_t)b * 2 * f + c];
@@ -122,13 +124,13 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restri
     red[ty][tx] = s;
     __syncthreads();
     if (ty == 0 && c < 2 * f) {
-        s = 0.f;
+        s = 0.0;
 #pragma unroll
         for (int i = 0; i < 64; ++i) s += red[i][tx];
         if (c < f) {
-            if (dweight) dweight[c] = s;
+            if (dweight) dweight[c] = (float)s;
         } else if (dbias) {
-            dbias[c - f] = s;
+            dbias[c - f] = (float)s;
         }
     }
 }
@@ -137,18 +139,18 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(const float *__restri
 // 512 floats: 5 us, and 5 us for the other kernel behind it; that one alone would have them in 32 workgroups).
 __global__ __launch_bounds__(256) void norm_params_chunk_kernel(const float *__restrict__ partial, int blocks, int f,
                                                                  float *__restrict__ out) {
-    __shared__ float red[4][64];
+    __shared__ double red[4][64];
     const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
     const int c = blockIdx.x * 64 + tx, per = (blocks + kParamsChunks - 1) / kParamsChunks;
     const int first = blockIdx.y * per, last = std::min(blocks, first + per);
-    float s = 0.f;
+    double s = 0.0;
     if (c < 2 * f) {
 #pragma unroll 8
         for (int b = first + ty; b < last; b += 4) s += partial[(int64_t)b * 2 * f + c];
     }
     red[ty][tx] = s;
     __syncthreads();
-    if (ty == 0 && c < 2 * f) out[(int64_t)blockIdx.y * 2 * f + c] = (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+    if (ty == 0 && c < 2 * f) out[(int64_t)blockIdx.y * 2 * f + c] = (float)((red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]));
 }
 
 bool known_type(int t) { return t == ROF_F32 || t == ROF_BF16; }

@@ -324,3 +324,16 @@ def test_a_batch_of_gradients_at_once():
         for i, dy in enumerate(batch):
             want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
             assert all(torch.equal(s[i], t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("n,step,tol", [(16384, 64, 1.0), (6400000, 256, 3.0)])
+def test_the_sums_over_workgroups_keep_small_terms_beside_a_large_one(n, step, tol):
+    """One row of 2^24 and ones, `step` rows apart, which is what a workgroup takes at a time: added up in 32 bits a one would be
+    lost beside 2^24.  In 64 bits what is left is half a step of 2^24, that is 1, for each time that a sum is stored: once, and
+    in a workgroup and a chunk of workgroups before that where the launch is tiles."""
+    x, (w, b) = rows(n, 16, 1), params(16, 2)
+    dy = torch.zeros(n, 16, device="cuda")
+    dy[::step] = 1.0
+    dy[0] = 2.0 ** 24
+    db, = torch.autograd.grad(layer_norm(x, w, b), b, dy)
+    assert (db.double() - (2.0 ** 24 + n // step - 1)).abs().max().item() <= tol
