@@ -240,7 +240,7 @@ struct RofDropoutBackward : public Node {
             at::NoGradGuard quiet;
             const Tensor rows = gradient_rows(grads[0], type);
             const at::AutoDispatchBelowADInplaceOrView below;
-            dx = dropout_op().call(rows, p, state, call);
+            dx = dropout_op().call(rows, p, maybe(state), call);
         }
         return once({dx}, "dropout");
     }
@@ -260,7 +260,7 @@ Tensor dropout_autograd(const Tensor &x, double p, const std::optional<Tensor> &
     if (at::GradMode::is_enabled() && x.requires_grad()) {
         auto node = std::shared_ptr<RofDropoutBackward>(new RofDropoutBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x));
-        node->rng = SavedVariable(*rng, false);
+        node->rng = SavedVariable(rng.value_or(Tensor()), false);
         node->p = p;
         node->call = call;
         node->type = x.scalar_type();

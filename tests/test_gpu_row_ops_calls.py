@@ -337,3 +337,36 @@ def test_the_sums_over_workgroups_keep_small_terms_beside_a_large_one(n, step, t
     dy[0] = 2.0 ** 24
     db, = torch.autograd.grad(layer_norm(x, w, b), b, dy)
     assert (db.double() - (2.0 ** 24 + n // step - 1)).abs().max().item() <= tol
+
+
+def test_a_mode_that_answers_for_the_operators():
+    """A dispatch mode may return what it likes without running them, also for arguments that they would refuse."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Answers(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return torch.empty_like(args[0]) if func is torch.ops.rof.dropout.default else func(*args, **(kwargs or {}))
+
+    x = rows(6, 8, 1).requires_grad_(True)
+    with Answers():
+        y = dropout(x, 0.5, None)
+    assert y.grad_fn is not None
+    with pytest.raises(RuntimeError, match="rng"):
+        y.sum().backward()
+
+
+def test_export_and_compile():
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = ROF_LayerNorm(24, relu=True)
+
+        def forward(self, x):
+            return self.norm(x * 2) + 1
+
+    net, x, dy = Net().cuda(), rows(6, 24, 1).requires_grad_(True), rows(6, 24, 2)
+    with pytest.raises(Exception, match="layer_norm"):
+        torch.export.export(net, (x.detach(),))
+    fast = torch.compile(net, backend="aot_eager")
+    assert torch.equal(fast(x), net(x))
+    assert torch.equal(torch.autograd.grad(fast(x), x, dy)[0], torch.autograd.grad(net(x), x, dy)[0])
