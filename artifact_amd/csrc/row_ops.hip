@@ -225,7 +225,10 @@ bool is_tiled(const NormShape &s, int64_t n) { return is_lean(s) && rounds_of(s,
 //   two, 512 workgroups    float32         1.01   1.09   1.09   1.15   1.20   1.26   1.28   1.27   1.26   1.26
 //     three vectors a lane bfloat16        0.86   0.96   0.95   0.95   0.96   0.96   0.97   0.97   0.97   0.98
 // So two rounds from kPairedRounds on, and five workgroups on a CU for one float32 vector from kFullRounds on.  Wide rows: two
-// rounds (20011 x 4099 bfloat16 with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71).
+// rounds (20011 x 4099 bfloat16 with four wavefronts: 106 us against 117 one at a time; forward with three 62 / 71) and two
+// workgroups on a CU (65 to 192 vectors, which are one wavefront's or less, nine widths and pairs of types at 8000 to 120000
+// rounds: 0.84 to 1.01 of the time that 1024 take), but four of those of two wavefronts (with ReLU and dropout 512 take 1.3 to
+// 1.75 times as long).
 int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
     const int64_t rows = s.rows(), rounds = rounds_of(s, a.n);
     const bool lean = is_lean(s), f32 = x_dtype == ROF_F32;
@@ -247,7 +250,7 @@ int norm_blocks(NormArgs &a, const NormShape &s, int x_dtype, bool backward) {
             most = s.k == 1 ? 1024 : 512;
     } else {
         a.inner = rounds < 2048 ? 1 : 2;
-        most = s.waves == 2 || s.lpr < 64 ? 1024 : 512;
+        most = s.waves == 2 ? 1024 : 512;
     }
     const int blocks = (int)std::min<int64_t>((rounds + a.inner - 1) / a.inner, most);
     a.jump = ((int64_t)blocks * a.inner - (a.inner - 1)) * rows;
