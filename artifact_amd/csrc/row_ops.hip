@@ -210,7 +210,9 @@ bool is_tiled(const NormShape &s, int64_t n) { return is_lean(s) && rounds_of(s,
 // Backward: each workgroup leaves a row of partial sums.  With many rounds it is tiles of four adjacent ones, handed out as
 // others end: up to 16384 for float32 (10^6 x 200 424 us; 4096 tiles 471, 1280 workgroups that stay 478; 2.4 M x 100 512 / 564 /
 // 570), up to 4096 for bfloat16, whose workgroups are fewer on a CU (1.6 M x 300 602, 16384 tiles 653, 1024 that stay 602; 2.4 M x
-// 47 171 / 184 / 170; 2^22 x 256 1132 / 1119 / 1207), and more launches and traffic for their sums.  With fewer rounds
+// 47 171 / 184 / 170; 2^22 x 256 1132 / 1119 / 1207), and more launches and traffic for their sums.  kManyRounds is one number for four crossings (geometric
+// means over 15 widths and types): 80000 rounds for two float32 vectors a lane, 130000 for one, 140000 for three bfloat16 ones,
+// and between 250000 and 500000 for one, where tiles take 1.06 of the time at 100000 and 0.93 at 524288.  With fewer rounds
 // workgroups stay, as many as fit: four on a CU (1024), two (512) where a lane holds several bfloat16 vectors, whose registers
 // leave room for no more.  Rows of up to 64 vectors, a dozen widths with and without ReLU and dropout, geometric means of the
 // times against one round at a time with 1024 workgroups, by the number of rounds:
